@@ -49,6 +49,18 @@ class AttentionDesc(C.Structure):
     ]
 
 
+class PagedAttentionDesc(C.Structure):
+    """hexb_paged_attention_desc of include/hexb.h."""
+    _fields_ = [
+        ("Q", C.c_void_p), ("K_cache", C.c_void_p), ("V_cache", C.c_void_p), ("Out", C.c_void_p),
+        ("prefix_pages", C.c_void_p), ("block_table", C.c_void_p), ("seq_lens", C.c_void_p), ("q_offsets", C.c_void_p),
+        ("T", C.c_int64), ("B", C.c_int64), ("Hq", C.c_int64), ("Hkv", C.c_int64), ("D", C.c_int64),
+        ("num_pages", C.c_int64), ("page_size", C.c_int64), ("prefix_len", C.c_int64), ("table_width", C.c_int64),
+        ("table_stride", C.c_int64), ("max_q", C.c_int64),
+        ("strides", C.c_int64 * 10), ("sm_scale", C.c_float),
+    ]
+
+
 _i64, _vp, _f, _i = C.c_int64, C.c_void_p, C.c_float, C.c_int
 
 # name -> (restype, argtypes); mirrors include/hexb.h one to one.
@@ -82,6 +94,10 @@ PROTOTYPES = {
     "hexb_binary": (_i, [_i, _i, _vp, _vp, _vp, _i64, _vp]),
     "hexb_sum": (_i, [_i, _vp, _vp, _i64, _vp]),
     "hexb_rope": (_i, [_i, _vp, _vp, _i64, _i64, _i64, _i64, C.POINTER(_i64), C.POINTER(_i64), _f, _vp]),
+    "hexb_qk_norm_rope": (_i, [_i] + [_vp] * 7 + [_i64] * 4 + [C.POINTER(_i64), _i, _i, _f, _f, _vp]),
+    "hexb_kv_cache_append": (_i, [_i] + [_vp] * 7 + [_i64] * 5 + [C.POINTER(_i64), _i, _i, _i, _f, _f, _vp]),
+    "hexb_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedAttentionDesc)]),
+    "hexb_paged_attention_f16": (_i, [C.POINTER(PagedAttentionDesc), _vp, C.c_size_t, _vp]),
     "hexb_decoder_workspace_bytes": (C.c_size_t, [C.POINTER(DecoderConfig)]),
     "hexb_decoder_forward_f16": (_i, [C.POINTER(DecoderConfig), C.POINTER(DecoderWeights), _vp, _vp, _vp, C.c_size_t, _vp]),
     "hexb_decoder_forward_f16_noalloc": (_i, [C.POINTER(DecoderConfig), C.POINTER(DecoderWeights), _vp, _vp, _vp]),

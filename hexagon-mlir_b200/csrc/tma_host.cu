@@ -261,6 +261,8 @@ int attn_device_status_fetch_and_clear(int *out);
 int norm_device_status_fetch_and_clear(int *out);
 int softmax_device_status_fetch_and_clear(int *out);
 int embed_device_status_fetch_and_clear(int *out);
+int heads_device_status_fetch_and_clear(int *out);
+int paged_device_status_fetch_and_clear(int *out);
 
 }  // namespace hexb
 
@@ -268,14 +270,18 @@ extern "C" int hexb_device_status(int *out) {
   using namespace hexb;
   if (!out) return HEXB_ERR_BAD_ARG;
   HEXB_CUDA_OK(cudaDeviceSynchronize());
-  int v[6] = {0, 0, 0, 0, 0, 0};
+  int v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (int s = gemm_device_status_fetch_and_clear(&v[0])) return s;
   if (int s = attn_device_status_fetch_and_clear(&v[1])) return s;
   if (int s = norm_device_status_fetch_and_clear(&v[2])) return s;
   if (int s = softmax_device_status_fetch_and_clear(&v[3])) return s;
   if (int s = embed_device_status_fetch_and_clear(&v[4])) return s;
   if (int s = selftest_device_status_fetch_and_clear(&v[5])) return s;
-  *out = v[0] ? v[0] : v[1] ? v[1] : v[2] ? v[2] : v[3] ? v[3] : v[4] ? v[4] : v[5];
+  if (int s = heads_device_status_fetch_and_clear(&v[6])) return s;
+  if (int s = paged_device_status_fetch_and_clear(&v[7])) return s;
+  *out = 0;
+  for (int i = 7; i >= 0; --i)
+    if (v[i]) *out = v[i];
   return HEXB_OK;
 }
 

@@ -549,6 +549,179 @@ def rope(x, out, theta: float = 10000.0) -> None:
         out.copy_(od)
 
 
+def _lead(t: torch.Tensor, what: str):
+    """Strides of all but the last dimension (which must be 1); a dimension of one element counts as 0."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: innermost stride must be 1")
+    return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(t.dim() - 1)]
+
+
+def _rotary(what: str, D: int, rotary_dim, theta: float, positions, tokens: int) -> int:
+    """rotary_dim as the library takes it: 0 without positions, D by default."""
+    if positions is None:
+        if rotary_dim:
+            raise ValueError(f"{what}: a rotation needs positions")
+        return 0
+    rot = D if rotary_dim is None else int(rotary_dim)
+    if positions.dtype != torch.int64 or positions.shape != (tokens,) or not positions.is_contiguous():
+        raise ValueError(f"{what}: positions must be a contiguous int64 [tokens] vector")
+    if rot < 0 or rot > D or rot % 2 or not theta > 0:
+        raise ValueError(f"{what}: rotary_dim must be even and at most D, theta positive")
+    return rot
+
+
+def _gain(what: str, w, D: int, like: torch.Tensor):
+    if w is not None and (w.shape != (D,) or w.dtype != like.dtype or not w.is_contiguous()):
+        raise ValueError(f"{what}: a norm weight must be a contiguous [D] vector of the tensors' dtype")
+
+
+def qk_norm_rope(q, k, q_out, k_out, positions=None, q_weight=None, k_weight=None, eps: float = 1e-6,
+                 theta: float = 10000.0, rotary_dim=None, interleaved: bool = True) -> None:
+    """RMS norm of every query and key head, then the rotation of the token's position, in one pass:
+    out[t, h] = R(positions[t]) (x[t, h] * rsqrt(mean(x[t, h]^2) + eps) * weight).
+
+    q, q_out: [tokens, q_heads, D]; k, k_out: [tokens, kv_heads, D]; float16 or float32, any strides with a unit
+    innermost one (views of a fused q|k|v buffer), q_out may be q and k_out may be k.  positions: int64 [tokens],
+    None for no rotation.  The first rotary_dim (default D) elements are turned by position *
+    theta^(-2p / rotary_dim), pairs (2p, 2p+1) when interleaved -- as in ``rope`` -- else (p, p + rotary_dim/2).
+    Weights None: ones.  Composed from rms_norm_fwd_kernel (test/python/triton/test_rms_norm.py:37-63) and
+    rope_kernel (test/python/triton/test_rope.py:98-190)."""
+    lib = _lib.load()
+    if any(t is not None and t.device.type != "cuda" for t in (q, k, q_out, k_out, positions, q_weight, k_weight)):
+        return _stage(lambda q, k, q_out, k_out, positions, q_weight, k_weight: qk_norm_rope(
+            q, k, q_out, k_out, positions, q_weight, k_weight, eps, theta, rotary_dim, interleaved),
+            dict(q=q, k=k, q_out=q_out, k_out=k_out, positions=positions, q_weight=q_weight, k_weight=k_weight),
+            ("q_out", "k_out"))
+    dev = _same_place(q, k, q_out, k_out, positions, q_weight, k_weight)
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError("qk_norm_rope: expected q [tokens, q_heads, D] and k [tokens, kv_heads, D]")
+    if q_out.shape != q.shape or k_out.shape != k.shape or not (q.dtype == k.dtype == q_out.dtype == k_out.dtype):
+        raise ValueError("qk_norm_rope: outputs must have the inputs' shapes and dtype")
+    dt = _dt(q)
+    T, Hq, D = q.shape
+    rot = _rotary("qk_norm_rope", D, rotary_dim, theta, positions, T)
+    _gain("qk_norm_rope", q_weight, D, q)
+    _gain("qk_norm_rope", k_weight, D, k)
+    st = (C.c_int64 * 8)(*_lead(q, "q"), *_lead(k, "k"), *_lead(q_out, "q_out"), *_lead(k_out, "k_out"))
+    with _guard(dev):
+        check(lib.hexb_qk_norm_rope(dt, _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), _ptr(positions), _ptr(q_weight),
+                                    _ptr(k_weight), T, Hq, k.shape[1], D, st, rot, int(bool(interleaved)), float(theta),
+                                    float(eps), _stream(q)), "qk_norm_rope")
+
+
+def kv_cache_append(k, v, k_cache, v_cache, slots, positions=None, k_weight=None, k_norm=None, eps: float = 1e-6,
+                    theta: float = 10000.0, rotary_dim=None, interleaved: bool = True, check_slots: bool = False) -> None:
+    """Stores the keys and values of new tokens in a paged cache, the keys rotated (and normed) on the way.
+
+    k, v: [tokens, kv_heads, D]; caches: [num_pages, page_size, kv_heads, D], any strides with a unit innermost
+    one; slots: int64 [tokens], slot s is row s % page_size of page s // page_size.  A negative slot is padding
+    and stores nothing; slots that are not negative must be distinct.  positions None: no rotation (else as in
+    ``qk_norm_rope``); k_weight, or k_norm=True for unit gains: the keys' RMS norm first.
+
+    A slot outside the cache stores nothing and records HEXB_ERR_BAD_ARG in the device status word.
+    ``check_slots=True`` validates the slots first -- one device synchronisation -- and raises IndexError for
+    one outside the cache, ValueError for one that is named twice."""
+    lib = _lib.load()
+    if any(t is not None and t.device.type != "cuda" for t in (k, v, k_cache, v_cache, slots, positions, k_weight)):
+        return _stage(lambda k, v, k_cache, v_cache, slots, positions, k_weight: kv_cache_append(
+            k, v, k_cache, v_cache, slots, positions, k_weight, k_norm, eps, theta, rotary_dim, interleaved, check_slots),
+            dict(k=k, v=v, k_cache=k_cache, v_cache=v_cache, slots=slots, positions=positions, k_weight=k_weight),
+            ("k_cache", "v_cache"))
+    dev = _same_place(k, v, k_cache, v_cache, slots, positions, k_weight)
+    if k.dim() != 3 or k.shape != v.shape:
+        raise ValueError("kv_cache_append: expected k and v of one shape [tokens, kv_heads, D]")
+    T, H, D = k.shape
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or tuple(k_cache.shape[2:]) != (H, D):
+        raise ValueError("kv_cache_append: expected caches of one shape [num_pages, page_size, kv_heads, D]")
+    if not (k.dtype == v.dtype == k_cache.dtype == v_cache.dtype):
+        raise TypeError("kv_cache_append: k, v and the caches must share a dtype")
+    dt = _dt(k)
+    if slots.dtype != torch.int64 or slots.shape != (T,) or not slots.is_contiguous():
+        raise ValueError("kv_cache_append: slots must be a contiguous int64 [tokens] vector")
+    rot = _rotary("kv_cache_append", D, rotary_dim, theta, positions, T)
+    _gain("kv_cache_append", k_weight, D, k)
+    pages, page_size = k_cache.shape[:2]
+    if T and page_size < 1:
+        raise ValueError("kv_cache_append: the pages hold no slot")
+    if check_slots and T:
+        used = slots[slots >= 0]
+        if used.numel() and int(used.max()) >= pages * page_size:
+            raise IndexError(f"kv_cache_append: slot {int(used.max())} is outside the cache of {pages * page_size}")
+        if used.unique().numel() != used.numel():
+            raise ValueError("kv_cache_append: a slot is named twice")
+    st = (C.c_int64 * 10)(*_lead(k, "k"), *_lead(v, "v"), *_lead(k_cache, "k_cache"), *_lead(v_cache, "v_cache"))
+    norm = k_weight is not None if k_norm is None else bool(k_norm)
+    if k_weight is not None and not norm:
+        raise ValueError("kv_cache_append: a k_weight without the norm it belongs to")
+    with _guard(dev):
+        check(lib.hexb_kv_cache_append(dt, _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(slots),
+                                       _ptr(positions), _ptr(k_weight), T, H, D, pages, page_size, st, int(norm), rot,
+                                       int(bool(interleaved)), float(theta), float(eps), _stream(k)), "kv_cache_append")
+
+
+def shared_prefix_attention(q, k_cache, v_cache, out, prefix_pages=None, prefix_len: int = 0, block_table=None,
+                            seq_lens=None, q_offsets=None, max_q: int = 0, sm_scale=None) -> None:
+    """Attention of a batch whose sequences share a prefix, over a paged cache; the prefix is read once for all.
+
+    q, out: float16 [tokens, q_heads, D] (out may be q); caches: float16 [num_pages, page_size, kv_heads, D], any
+    strides with a unit innermost one; q_heads a multiple of kv_heads (query heads h*G .. h*G+G-1 read key head h);
+    D a multiple of 8, at most 256.  Sequence b has the tokens q_offsets[b] : q_offsets[b+1] (int32 [batch + 1],
+    from 0; None: one token each) and seq_lens[b] keys of its own (int32 [batch]), the last of them those of
+    its new tokens: token i of nq sees the prefix_len prefix keys and its own keys j <= seq_lens[b] - nq + i.  Own
+    key j is slot j % page_size of page block_table[b, j // page_size] (int32 [batch, width]); prefix keys lie in
+    prefix_pages (int32) the same way.  A token that sees no key gets zeros; rows from q_offsets[-1] on are left as
+    they are.  max_q: the usual number of new tokens of a sequence -- it shapes the launch, any value is right.
+
+    Lengths, tables and offsets stay on the device and are read by every launch, so a captured CUDA graph
+    follows them; only prefix_len and the shapes are fixed at capture.  A page outside the cache reads as zeros, a
+    length beyond the table is cut; both record HEXB_ERR_BAD_ARG in the device status word.
+    The softmax and its scale are those of ``attention`` (test/python/triton/test_flash_attention.py:37-168)."""
+    lib = _lib.load()
+    every = dict(q=q, k_cache=k_cache, v_cache=v_cache, out=out, prefix_pages=prefix_pages, block_table=block_table,
+                 seq_lens=seq_lens, q_offsets=q_offsets)
+    if any(t is not None and t.device.type != "cuda" for t in every.values()):
+        return _stage(lambda q, k_cache, v_cache, out, prefix_pages, block_table, seq_lens, q_offsets:
+                      shared_prefix_attention(q, k_cache, v_cache, out, prefix_pages, prefix_len, block_table, seq_lens,
+                                              q_offsets, max_q, sm_scale), every, ("out",))
+    dev = _same_place(*every.values())
+    if q.dim() != 3 or out.shape != q.shape:
+        raise ValueError("shared_prefix_attention: expected q and out of one shape [tokens, q_heads, D]")
+    T, Hq, D = q.shape
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != D:
+        raise ValueError("shared_prefix_attention: expected caches of one shape [num_pages, page_size, kv_heads, D]")
+    if not (q.dtype == out.dtype == k_cache.dtype == v_cache.dtype == torch.float16):
+        raise TypeError("shared_prefix_attention: float16 tensors expected")
+    pages, page_size, Hkv, _ = k_cache.shape
+    if Hkv == 0 or Hq % Hkv or page_size < 1:
+        raise ValueError("shared_prefix_attention: q_heads must be a multiple of kv_heads, page_size positive")
+    for name, t, dim in (("prefix_pages", prefix_pages, 1), ("block_table", block_table, 2), ("seq_lens", seq_lens, 1),
+                         ("q_offsets", q_offsets, 1)):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != dim or (t.numel() > 1 and t.stride(-1) != 1)):
+            raise ValueError(f"shared_prefix_attention: {name} must be int32 with {dim} dimension(s) and unit stride")
+    if prefix_len < 0 or max_q < 0 or (prefix_len and (prefix_pages is None or prefix_pages.numel() * page_size < prefix_len)):
+        raise ValueError("shared_prefix_attention: prefix_pages do not hold prefix_len keys")
+    if (block_table is None) != (seq_lens is None):
+        raise ValueError("shared_prefix_attention: block_table and seq_lens belong together")
+    B = q_offsets.numel() - 1 if q_offsets is not None else T
+    if B < 0 or (block_table is not None and (block_table.shape[0] != B or seq_lens.numel() != B)):
+        raise ValueError("shared_prefix_attention: block_table, seq_lens and q_offsets disagree about the batch")
+    d = _lib.PagedAttentionDesc()
+    d.Q, d.K_cache, d.V_cache, d.Out = _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out)
+    d.prefix_pages, d.q_offsets = _ptr(prefix_pages), _ptr(q_offsets)
+    d.T, d.B, d.Hq, d.Hkv, d.D = T, B, Hq, Hkv, D
+    d.num_pages, d.page_size, d.prefix_len, d.max_q = pages, page_size, prefix_len, max_q
+    if block_table is not None:
+        d.block_table, d.seq_lens = _ptr(block_table), _ptr(seq_lens)
+        d.table_width, d.table_stride = block_table.shape[1], block_table.stride(0)
+    d.strides = (C.c_int64 * 10)(*_lead(q, "q"), *_lead(k_cache, "k_cache"), *_lead(v_cache, "v_cache"), *_lead(out, "out"))
+    d.sm_scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    with _guard(dev):
+        need = lib.hexb_paged_attention_workspace_bytes(C.byref(d))
+        # from torch's allocator: its blocks follow the stream, and a captured graph keeps its own
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        check(lib.hexb_paged_attention_f16(C.byref(d), _ptr(ws), need, _stream(q)), "shared_prefix_attention")
+
+
 class DecoderStack:
     """The decoder-only block stack on one GPU: holds the weight pointer tables and the workspace.
 

@@ -267,6 +267,63 @@ int hexb_decoder_forward_f16(const hexb_decoder_config *cfg, const hexb_decoder_
 int hexb_decoder_forward_f16_noalloc(const hexb_decoder_config *cfg, const hexb_decoder_weights *w,
                                      const void *x, void *out, void *stream);
 
+/* ---- serving step over a paged key/value cache.  The reference compiles whole prompts only (its GPT-2 test,
+ * test/python/torch-mlir/gpt2lmheadmodel.py:143-169, has no cache); these entry points add the step that answers
+ * token by token, next to rope_kernel, rms_norm_fwd_kernel, attention_fwd_kernel and softmax_kernel above.
+ * A cache is [num_pages, page_size, kv_heads, D] with any strides (innermost 1); slot s of it is row s % page_size
+ * of page s / page_size. */
+
+/* Per-head RMS norm of queries and keys and the rotation of their positions, one pass:
+ *   out[t, h, :] = R(positions[t]) . (x[t, h, :] * rsqrt(mean(x[t, h, :]^2) + eps) * weight)
+ * q, q_out [tokens, q_heads, D] and k, k_out [tokens, kv_heads, D]; strides[8] = (token, head) of q, k, q_out,
+ * k_out in elements (innermost 1).  q_weight / k_weight [D], NULL for ones.  R turns the pairs of the first
+ * rotary_dim elements (even, <= D and <= 512; 0: no rotation, positions may be NULL) by position *
+ * theta^(-2p / rotary_dim): pair (2p, 2p+1) when interleaved != 0 (the convention of hexb_rope), else
+ * (p, p + rotary_dim/2).  q_out may be q, and k_out k (same strides); other overlaps are not allowed. D <= 4096. */
+int hexb_qk_norm_rope(int dtype, const void *q, const void *k, void *q_out, void *k_out, const int64_t *positions,
+                      const void *q_weight, const void *k_weight, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                      int64_t D, const int64_t *strides, int rotary_dim, int interleaved, float theta, float eps,
+                      void *stream);
+
+/* Stores new keys and values in their cache slots: k_cache[slots[t]] = R . norm(k[t]), v_cache[slots[t]] = v[t].
+ * k, v [tokens, kv_heads, D]; strides[10] = (token, head) of k, (token, head) of v, (page, slot, head) of k_cache
+ * and of v_cache.  k_norm != 0 applies the norm of hexb_qk_norm_rope to the keys (k_weight NULL: ones);
+ * rotary_dim, interleaved, theta, positions as there.  A negative slot stores nothing (padding); one outside the
+ * cache stores nothing and makes hexb_device_status report HEXB_ERR_BAD_ARG.  Slots that are not negative must
+ * be distinct: a slot named twice holds some mixture of its rows.  The caches must not overlap k, v or each other. */
+int hexb_kv_cache_append(int dtype, const void *k, const void *v, void *k_cache, void *v_cache, const int64_t *slots,
+                         const int64_t *positions, const void *k_weight, int64_t tokens, int64_t kv_heads, int64_t D,
+                         int64_t num_pages, int64_t page_size, const int64_t *strides, int k_norm, int rotary_dim,
+                         int interleaved, float theta, float eps, void *stream);
+
+/* Attention of a batch that shares a prefix, fp16 (the softmax of hexb_attention_fwd_f16).  Query token i of the
+ * nq new tokens of sequence b sees the keys 0 .. prefix_len-1 of the shared prefix and the keys
+ * j <= seq_lens[b] - nq + i of its own pages (the new tokens' keys are its last nq):
+ *   Out = softmax(Q . K^T * sm_scale) . V over their union.
+ * A query that sees no key yields zeros.  Q, Out [T, Hq, D]; D a multiple of 8, at most 256; Hq a multiple of Hkv,
+ * query heads h*G .. h*G+G-1 (G = Hq / Hkv) read key head h.  Sequence b owns tokens q_offsets[b] ..
+ * q_offsets[b+1]-1 (int32 [B+1] from 0, ascending; NULL: one token each, T == B); rows from q_offsets[B] on are
+ * left as they are.  Key j of sequence b is slot j % page_size of page block_table[b, j / page_size]
+ * (int32 [B, table_width], row stride table_stride), key j of the prefix likewise through prefix_pages
+ * (ceil(prefix_len / page_size) entries).  table_width 0: no own keys; prefix_len 0: no prefix.  Lengths, tables and
+ * offsets are read on the device by every launch, so a captured graph follows them; a page outside the cache
+ * reads as zeros, a length beyond the table is cut, and both make hexb_device_status report HEXB_ERR_BAD_ARG.
+ * max_q: the usual number of new tokens of a sequence, for the launch shape only (0: T / B); any value is right.
+ * Q, Out, caches: 16-byte aligned, strides multiples of 8 elements.  Out may be Q.
+ * The workspace (see the query; 0 bytes: none) holds nothing between calls; calls that overlap need their own. */
+typedef struct hexb_paged_attention_desc {
+  const void *Q, *K_cache, *V_cache;
+  void *Out;
+  const int32_t *prefix_pages, *block_table, *seq_lens, *q_offsets;
+  int64_t T, B, Hq, Hkv, D;
+  int64_t num_pages, page_size, prefix_len, table_width, table_stride, max_q;
+  int64_t strides[10];       /* Q (token, head); K_cache (page, slot, head); V_cache likewise; Out (token, head) */
+  float sm_scale;
+} hexb_paged_attention_desc;
+size_t hexb_paged_attention_workspace_bytes(const hexb_paged_attention_desc *desc);
+int hexb_paged_attention_f16(const hexb_paged_attention_desc *desc, void *workspace, size_t workspace_bytes,
+                             void *stream);
+
 /* ---- host-buffer entry points (the launcher path).  Replace the generated wrapper main() that
  * loads `<kernel>_t{i}.raw`, runs the kernel and dumps `<kernel>_o{i}.raw`
  * (qcom_hexagon_backend/backend/triton_hexagon_launcher.py:111-123,
