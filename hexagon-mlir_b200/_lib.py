@@ -98,6 +98,7 @@ PROTOTYPES = {
     "hexb_kv_cache_append": (_i, [_i] + [_vp] * 7 + [_i64] * 5 + [C.POINTER(_i64), _i, _i, _i, _f, _f, _vp]),
     "hexb_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedAttentionDesc)]),
     "hexb_paged_attention_f16": (_i, [C.POINTER(PagedAttentionDesc), _vp, C.c_size_t, _vp]),
+    "hexb_sample_tokens": (_i, [_i] + [_vp] * 3 + [_i64] * 3 + [_vp] * 4 + [_f, _i, _f, _f, _vp]),
     "hexb_decoder_workspace_bytes": (C.c_size_t, [C.POINTER(DecoderConfig)]),
     "hexb_decoder_forward_f16": (_i, [C.POINTER(DecoderConfig), C.POINTER(DecoderWeights), _vp, _vp, _vp, C.c_size_t, _vp]),
     "hexb_decoder_forward_f16_noalloc": (_i, [C.POINTER(DecoderConfig), C.POINTER(DecoderWeights), _vp, _vp, _vp]),

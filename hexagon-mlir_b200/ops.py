@@ -722,6 +722,47 @@ def shared_prefix_attention(q, k_cache, v_cache, out, prefix_pages=None, prefix_
         check(lib.hexb_paged_attention_f16(C.byref(d), _ptr(ws), need, _stream(q)), "shared_prefix_attention")
 
 
+def sample_tokens(logits, u, out, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> None:
+    """out[r] = one token of logits[r], drawn with the given random number u[r] in [0, 1).
+
+    logits: float16 or float32 [rows, vocab], unit inner stride; u: float32 [rows]; out: int64 [rows].  Each parameter
+    is a number or a tensor of one value per row (float32; top_k int32).  With w_i = exp((x_i - max x) / temperature):
+    top_k > 0 keeps the k largest logits, top_p < 1 of those, in descending order, every one before which less than
+    top_p of their mass lies, min_p > 0 of those the ones with w_i >= min_p; the token is the first kept index, in
+    index order, whose inclusive sum of w exceeds u times the kept sum.  temperature 0: the largest logit.
+    Ties go to the lowest index.  NaN and -inf are never chosen; a row of nothing else gives -1."""
+    lib = _lib.load()
+    tens = lambda v: v if torch.is_tensor(v) else None
+    every = dict(logits=logits, u=u, out=out, temperature=tens(temperature), top_k=tens(top_k), top_p=tens(top_p),
+                 min_p=tens(min_p))
+    if any(t is not None and t.device.type != "cuda" for t in every.values()):
+        pick = lambda a, b: b if a is None else a
+        return _stage(lambda logits, u, out, **k: sample_tokens(
+            logits, u, out, pick(k["temperature"], temperature), pick(k["top_k"], top_k), pick(k["top_p"], top_p),
+            pick(k["min_p"], min_p)), every, ("out",))
+    dev = _same_place(*every.values())
+    rows, vocab, xs = _rows2d(logits, "logits")
+    dt = _dt(logits)
+    if vocab < 1:
+        raise ValueError("sample_tokens: no logits to choose from")
+    if u.dtype != torch.float32 or out.dtype != torch.int64:
+        raise TypeError("sample_tokens: u must be float32 and out int64")
+    for name, t, kind in (("u", u, u.dtype), ("out", out, out.dtype), ("temperature", every["temperature"], torch.float32),
+                          ("top_k", every["top_k"], torch.int32), ("top_p", every["top_p"], torch.float32),
+                          ("min_p", every["min_p"], torch.float32)):
+        if t is not None and (t.shape != (rows,) or t.dtype != kind or not t.is_contiguous()):
+            raise ValueError(f"sample_tokens: {name} must be a contiguous {kind} [rows] vector")
+    num = lambda name, v, off: off if every[name] is not None else v
+    t0, k0, p0, m0 = (num("temperature", temperature, 0.0), num("top_k", top_k, 0), num("top_p", top_p, 1.0),
+                      num("min_p", min_p, 0.0))
+    if not (t0 >= 0 and k0 >= 0 and 0 <= p0 <= 1 and 0 <= m0 <= 1):
+        raise ValueError("sample_tokens: temperature and top_k must not be negative, top_p and min_p lie in [0, 1]")
+    with _guard(dev):
+        check(lib.hexb_sample_tokens(dt, _ptr(logits), _ptr(u), _ptr(out), rows, vocab, xs, _ptr(every["temperature"]),
+                                     _ptr(every["top_k"]), _ptr(every["top_p"]), _ptr(every["min_p"]), float(t0),
+                                     min(int(k0), 0x7fffffff), float(p0), float(m0), _stream(logits)), "sample_tokens")
+
+
 class DecoderStack:
     """The decoder-only block stack on one GPU: holds the weight pointer tables and the workspace.
 

@@ -49,8 +49,9 @@ const char *hexb_status_string(int status);
 /* Text of the last CUDA error seen by this thread inside the library ("" if none). */
 const char *hexb_last_cuda_error(void);
 /* Synchronises the current device, then reports and clears the sticky device-side status word
- * that bounded waits inside the tensor-core kernels set when they give up.  *out = HEXB_OK or
- * HEXB_ERR_TIMEOUT.  Replaces: DMAStatus out-param of the UserDMA runtime
+ * that bounded waits inside the tensor-core kernels set when they give up, and that kernels set for
+ * indexes outside their tables (token ids, cache slots and pages).  *out = HEXB_OK, HEXB_ERR_TIMEOUT or
+ * HEXB_ERR_BAD_ARG.  Replaces: DMAStatus out-param of the UserDMA runtime
  * (qcom_hexagon_backend/bin/runtime/include/RuntimeDMA.h:18). */
 int hexb_device_status(int *out);
 /* Self-test of that mechanism: launches one small CTA (producer / TMEM owner / consumer warps as in
@@ -323,6 +324,22 @@ typedef struct hexb_paged_attention_desc {
 size_t hexb_paged_attention_workspace_bytes(const hexb_paged_attention_desc *desc);
 int hexb_paged_attention_f16(const hexb_paged_attention_desc *desc, void *workspace, size_t workspace_bytes,
                              void *stream);
+
+/* One token per row of logits [rows, vocab] (fp16 or fp32, row stride in elements, rows of any alignment), from a
+ * given uniform random number u[row] in [0, 1).  With w_i = exp((x_i - max x) / T):
+ *   T <= 0        out = the lowest index of the largest logit;
+ *   top_k > 0     keeps the k largest logits (0: all);
+ *   top_p < 1     keeps, in descending order, every one before which less than top_p of the mass left by top_k lies
+ *                 (at least the first);
+ *   min_p > 0     keeps those with w_i >= min_p (at most 1 counts);
+ *   out = the first kept index, in index order, whose inclusive sum of w exceeds u * (sum of the kept w).
+ * Ties rank by index, the lower one first.  NaN and -inf are never chosen; a row of nothing else gives -1.
+ * +inf: only the rows' +inf entries have weight.  u outside [0, 1) is clamped.  Weights and sums are formed in 64 bits, and
+ * the result does not depend on the order of atomics.  The parameters are device arrays of `rows` entries, or NULL
+ * for the scalar that follows (temperature0, ...).  vocab <= 2^28. */
+int hexb_sample_tokens(int dtype, const void *logits, const float *u, int64_t *out, int64_t rows, int64_t vocab,
+                       int64_t row_stride, const float *temperature, const int32_t *top_k, const float *top_p,
+                       const float *min_p, float temperature0, int top_k0, float top_p0, float min_p0, void *stream);
 
 /* ---- host-buffer entry points (the launcher path).  Replace the generated wrapper main() that
  * loads `<kernel>_t{i}.raw`, runs the kernel and dumps `<kernel>_o{i}.raw`

@@ -119,3 +119,26 @@ def test_python_checks_of_the_attention():
             call(**bad)
     with pytest.raises(TypeError):
         call(q=meta(4, 8, 64, dtype=torch.float32), out=meta(4, 8, 64, dtype=torch.float32))
+
+
+def test_sample_tokens_refusals():
+    lib = hexb200.load()
+    call = lambda dt=2, ptr=64, rows=4, V=100, st=100, u=64: lib.hexb_sample_tokens(
+        dt, ptr, u, 64, rows, V, st, None, None, None, None, 1.0, 0, 1.0, 0.0, None)
+    assert call(dt=6) == -2 and call(rows=-1) == -1 and call(V=0) == -1 and call(st=-1) == -1 and call(rows=0) == 0
+    assert call(ptr=None) == -1 and call(u=None) == -1 and call(ptr=66) == -3 and call(V=1 << 29) == -2
+    x, u, out = meta(4, 100), meta(4, dtype=torch.float32), meta(4, dtype=torch.int64)
+    for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_k=-1), dict(top_p=1.5), dict(top_p=-0.1),
+                dict(min_p=2.0)):
+        with pytest.raises(ValueError):
+            ops.sample_tokens(x, u, out, **bad)
+    with pytest.raises(ValueError):
+        ops.sample_tokens(x, meta(5, dtype=torch.float32), out)
+    with pytest.raises(ValueError):
+        ops.sample_tokens(meta(4, 0), u, out)
+    with pytest.raises(ValueError):
+        ops.sample_tokens(meta(400), u, out)
+    with pytest.raises(TypeError):
+        ops.sample_tokens(x, u, meta(4, dtype=torch.int32))
+    with pytest.raises(TypeError):
+        ops.sample_tokens(meta(4, 100, dtype=torch.bfloat16), u, out)
