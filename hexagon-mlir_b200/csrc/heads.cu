@@ -14,9 +14,8 @@
 // is a few shuffles; the sines and cosines depend on (token, pair) only and are computed once per CTA
 // into shared memory, then used by all heads of its tokens.
 //
-// The angle of a far position: pos * frequency is formed in 64 bits and reduced to a fraction of a turn before
-// it is rounded to 32 (at position 130000 a 32-bit product is off by up to 2^-24 * 130000 = 0.008 rad); the
-// frequencies, in turns, come as 64-bit kernel parameters computed by the host.
+// The angle of a far position: a 32-bit product of position and frequency is off by up to 2^-24 * 130000 = 0.008 rad
+// at position 130000, so it is formed in 64-bit fixed point and rounded to 32 bits as a fraction of a turn.
 #include <cmath>
 
 #include "common.cuh"
@@ -27,12 +26,8 @@ static __device__ int g_heads_status = 0;
 
 namespace heads {
 
-constexpr int kMaxPairs = 256;  // rotary_dim <= 512: the frequency table travels as a kernel parameter
-constexpr int THREADS = 256;
-
-struct Freqs {
-  double turns[kMaxPairs];  // theta^(-2p / rotary_dim) / (2 pi)
-};
+constexpr int THREADS = 128;
+constexpr int kPowerBits = 11;   // rotary_dim <= 4096
 
 // One of the two tensors a call walks (queries and keys, or keys and values).
 struct Segment {
@@ -52,16 +47,31 @@ struct Params {
   const int64_t *slots;       // NULL: destination rows follow the tokens
   int64_t tokens, num_slots, page_size;
   int D, rot, interleaved;
-  int tokens_per_cta, rows_per_split;
+  int tokens_per_cta, gpt_shift;   // groups of lanes a token has: 1 << gpt_shift
   float eps;
+  uint64_t power[kPowerBits];
 };
 
+// Angles are fractions of a turn in 64-bit fixed point: 2^64 is one turn, a product with the position wraps as an
+// angle does, and no 64-bit floating-point chain delays the first row of a CTA (with one, a single token took
+// 6.0 us against 3.3).  The frequency of pair p is 2^64 / (2 pi) * theta^(-2p / rotary_dim): the product of the powers
+// theta^(-2^(b+1) / rotary_dim) over the bits b of p, which the host forms in 64-bit floating point (2^63 is 1):
+// relative error at most 12 * 2^-53, so the angle at position n is good to n * 2^-50 of a turn.
+__device__ __forceinline__ uint64_t frequency(const Params &p, int pr) {
+  uint64_t f = 2935890503282001226ull;  // 2^64 / (2 pi)
+#pragma unroll
+  for (int b = 0; b < kPowerBits; ++b) {
+    if ((p.rot - 1) >> (b + 1) == 0) break;
+    const uint64_t g = __umul64hi(f, p.power[b]) << 1;
+    f = pr >> b & 1 ? g : f;
+  }
+  return f;
+}
 // cos and sin of pos * frequency
-__device__ __forceinline__ float2 turn(int64_t pos, double freq_turns) {
-  double t = (double)pos * freq_turns;
-  t -= rint(t);
+__device__ __forceinline__ float2 turn(int64_t pos, uint64_t freq) {
+  const int32_t t = (int32_t)(((uint64_t)pos * freq) >> 32);
   float sn, cs;
-  sincospif(2.0f * (float)t, &sn, &cs);
+  sincospif((float)t * 4.656612873077393e-10f, &sn, &cs);  // 2^-31: half turns
   return make_float2(cs, sn);
 }
 
@@ -85,147 +95,186 @@ __device__ __forceinline__ int64_t load_slot(const Params &p, int64_t token) {
   return slot;
 }
 
-// Vector form.  LPR lanes hold one row, NV 16-byte vectors each (vector v sits in lane v % LPR, register
-// v / LPR).  grid.x: blocks of tokens_per_cta tokens; grid.y: splits of a token's rows (few tokens only).
+// Vector form.  LPR lanes hold one row, NV 16-byte vectors each (vector v sits in lane v % LPR, register v / LPR).
+// A CTA takes tokens_per_cta tokens; a token's heads (of both tensors, in one row) are dealt to 1 << gpt_shift groups
+// of lanes.  Instruction issue, not memory, bounds this kernel (350 instructions a row with the addresses and the
+// rotation formed anew for each: 80 us where the traffic takes 21), so what the rows of a group share is set up
+// once: the addresses advance by a constant, and the linear map of a row
+//   y_e = rstd * (A_e x_e + B_e x_partner(e)),   A = w cos,  B = -+ w_partner sin
+// sits in registers -- two fused operations an element besides the mean.  The first row is requested before the
+// angles are computed, and the next while one is worked on.  The code is kept to one copy of each step: with
+// few tokens the time is that of fetching it.
 template <typename T, int LPR, int NV>
-__global__ void __launch_bounds__(THREADS)
-head_rows_kernel(const Params p, const __grid_constant__ Freqs fr) {
+__global__ void __launch_bounds__(THREADS, 5)
+head_rows_kernel(const Params p) {
   constexpr int E = Vec16<T>::N;
   using Raw = decltype(Vec16<T>::raw);
-  constexpr int RP = THREADS / LPR;  // rows at a time
-  extern __shared__ float2 s_cs[];   // [tokens_per_cta][rot / 2]
+  // cos, sin of pair (v, e) of vector v at [token][e][v]: the lanes of a row read consecutive words
+  extern __shared__ float2 s_cs[];
   const int lane = threadIdx.x % LPR, grp = threadIdx.x / LPR;
-  const int nvec = p.D / E, half = p.rot / 2;
-  const int64_t t0 = (int64_t)blockIdx.x * p.tokens_per_cta;
+  const int nvec = p.D / E, half = p.rot / 2, rotv = p.rot / E, hv = half / E;
+  const bool inter = p.interleaved != 0;
+  const unsigned mask = LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1u) << ((threadIdx.x & 31) / LPR * LPR);
+  const int gs = p.gpt_shift, gpt = 1 << gs;
+  const int t = grp >> gs, h0 = grp & (gpt - 1), h1 = (h0 - p.seg[0].heads) & (gpt - 1);
+  const int64_t t0 = (int64_t)blockIdx.x * p.tokens_per_cta, tok = t0 + t;
   const int nt = (int)min((int64_t)p.tokens_per_cta, p.tokens - t0);
-  const int heads = p.seg[0].heads + p.seg[1].heads;
-  const int r_lo = (int)blockIdx.y * p.rows_per_split;
-  const int r_hi = min(r_lo + p.rows_per_split, nt * heads);
+  const int pairs_v = inter ? E / 2 : E, width = half / pairs_v, plane = pairs_v * width;
+  const int n0 = t < nt && h0 < p.seg[0].heads ? (p.seg[0].heads - h0 + gpt - 1) >> gs : 0;
+  const int n1 = t < nt && h1 < p.seg[1].heads ? (p.seg[1].heads - h1 + gpt - 1) >> gs : 0;
   pdl_wait();
-  if (p.rot) {
-    for (int i = threadIdx.x; i < nt * half; i += THREADS) {
-      const int t = i / half, pr = i - t * half;
-      s_cs[i] = turn(p.positions[t0 + t], fr.turns[pr]);
-    }
-  }
-  // gains of this lane's columns
-  Raw w[2][NV];
-#pragma unroll
-  for (int g = 0; g < 2; ++g)
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = lane + i * LPR;
-      if (p.seg[g].norm && p.seg[g].weight && v < nvec)
-        w[g][i] = *(reinterpret_cast<const Raw *>(p.seg[g].weight) + v);
-    }
-  __syncthreads();
-  const float inv_d = 1.0f / (float)p.D;
-  for (int r = r_lo + grp; r < r_hi; r += RP) {
-    const int t = r / heads;
-    int h = r - t * heads;
-    const int g = h >= p.seg[0].heads;
-    if (g) h -= p.seg[0].heads;
-    const Segment &s = p.seg[g];
-    const int64_t slot = p.slots ? load_slot(p, t0 + t) : 0;
-    const T *src = static_cast<const T *>(s.src) + (t0 + t) * s.src_t + (int64_t)h * s.src_h;
-    float f[NV][E];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = lane + i * LPR;
-      if (v < nvec) {
-        Vec16<T> x;
-        x.raw = ld_stream_as<Raw>(src + v * E);
-        x.unpack(f[i]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) f[i][e] = 0.f;
-      }
-    }
-    // lanes of one row take the same branches: a group of LPR lanes shares (t, h)
-    const unsigned mask = LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1u) << ((threadIdx.x & 31) / LPR * LPR);
-    if (s.norm) {
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < E; ++e) ss = fmaf(f[i][e], f[i][e], ss);
-#pragma unroll
-      for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-      const float rstd = rsqrtf(fmaf(ss, inv_d, p.eps));
+
+  const T *src = static_cast<const T *>(p.seg[0].src) + tok * p.seg[0].src_t + (int64_t)h0 * p.seg[0].src_h + lane * E;
+  const T *src1 = static_cast<const T *>(p.seg[1].src) + tok * p.seg[1].src_t + (int64_t)h1 * p.seg[1].src_h + lane * E;
+  Raw raw[NV];
+  auto request = [&](int n) {
+    if (n < n0 + n1) {
+      if (n == n0) src = src1;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        float wf[E];
-        if (s.weight) {
+        raw[i] = Raw{};
+        if (lane + i * LPR < nvec) raw[i] = ld_stream_as<Raw>(src + i * LPR * E);
+      }
+      src += p.seg[n >= n0].src_h << gs;
+    }
+  };
+  request(0);
+  // the gains are needed after the angles: their fetch overlaps that of the positions (one token: 6.7 -> 6.2 us)
+  if (threadIdx.x < 2 * LPR * NV) {
+    const int g = threadIdx.x >= LPR * NV, v = threadIdx.x - g * LPR * NV;
+    const Segment &s = p.seg[g];
+    if (s.norm && s.weight && v < nvec)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const T *>(s.weight) + v * E));
+  }
+  const int64_t slot = p.slots && t < nt ? load_slot(p, tok) : 0;
+  if (p.rot) {
+    // a thread keeps its pair and steps over tokens while the pairs are fewer than the threads
+    const int lanes = half < THREADS ? THREADS / half * half : THREADS;
+    for (int pr = threadIdx.x < lanes ? threadIdx.x % half : half; pr < half; pr += THREADS) {
+      const uint64_t fq = frequency(p, pr);
+      for (int ti = threadIdx.x / half; ti < nt; ti += max(1, lanes / half))
+        s_cs[ti * plane + pr % pairs_v * width + pr / pairs_v] = turn(p.positions[t0 + ti], fq);
+    }
+    __syncthreads();
+  }
+  const float2 *cs = s_cs + t * plane;
+  const float inv_d = 1.0f / (float)p.D;
+
+  float A[NV][E], B[NV][E];
+  T *dst = nullptr;
+  bool norm = false, rotate = false;
+  int64_t dst_step = 0;
+#pragma unroll 1
+  for (int n = 0; n < n0 + n1; ++n) {
+    if (n == 0 || n == n0) {
+      const int g = n >= n0;
+      const Segment &s = p.seg[g];
+      norm = s.norm;
+      rotate = s.rotate;
+      dst_step = s.dst_h << gs;
+      dst = dst_row<T>(s, p, tok, slot, g ? h1 : h0);
+      if (!dst) dst_step = 0;
+      else dst += lane * E;
+      const Raw *w = norm ? static_cast<const Raw *>(s.weight) : nullptr;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = lane + i * LPR;
+        const int pv = inter ? v : v < hv ? v + hv : v - hv;
+        const bool turned = rotate && v < rotv;
+        float wp[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) A[i][e] = wp[e] = 1.0f;
+        if (w && v < nvec) {
           Vec16<T> x;
-          x.raw = g ? w[1][i] : w[0][i];
-          x.unpack(wf);
+          x.raw = w[v];
+          x.unpack(A[i]);
+          if (turned) x.raw = w[pv];
+          x.unpack(wp);
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) f[i][e] *= s.weight ? rstd * wf[e] : rstd;
+        for (int e = 0; e < E; ++e) {
+          const float sign = (inter ? (e & 1) == 0 : v < hv) ? -1.0f : 1.0f;
+          float2 c = make_float2(1.0f, 0.0f);
+          if (turned) c = cs[inter ? e / 2 * width + v : e * width + min(v, pv)];
+          A[i][e] *= c.x;
+          B[i][e] = sign * (inter ? wp[e ^ 1] : wp[e]) * c.y;
+        }
       }
     }
-    if (s.rotate) {
-      const float2 *cs = s_cs + t * half;
-      if (p.interleaved) {
+    if (!norm && !rotate) {  // values: the bits as they are
+      if (dst) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int p0 = (lane + i * LPR) * (E / 2);
+        for (int i = 0; i < NV; ++i)
+          if (lane + i * LPR < nvec) st_stream_as<Raw>(dst + i * LPR * E, raw[i]);
+      }
+      request(n + 1);
+    } else {
+      float f[NV][E], o[NV][E];
 #pragma unroll
-          for (int e = 0; e < E / 2; ++e) {
-            if (p0 + e < half) {
-              const float2 c = cs[p0 + e];
-              const float a = f[i][2 * e], b = f[i][2 * e + 1];
-              f[i][2 * e] = a * c.x - b * c.y;
-              f[i][2 * e + 1] = a * c.y + b * c.x;
-            }
-          }
-        }
+      for (int i = 0; i < NV; ++i) {
+        Vec16<T> x;
+        x.raw = raw[i];
+        x.unpack(f[i]);
+      }
+      if (inter) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[i][e] = f[i][e ^ 1];
+      } else if (hv == LPR) {
+        // a lane holds both vectors of its pairs (the whole of a row of LPR * NV vectors is rotated)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[i][e] = f[NV - 1 - i][e];
       } else {
-        // the partner of vector v is v + half / E (first half) or v - half / E (second half)
-        const int hv = half / E;
-        float o[NV][E];
+        // the partner of vector v is v + hv (first half) or v - hv (second half)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int v = lane + i * LPR;
           const int pv = v < hv ? v + hv : v - hv;
           const int pl = pv & (LPR - 1), pi = pv / LPR;
+          uint32_t w[4];
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            float q = __shfl_sync(mask, f[0][e], pl, LPR);
-            if (NV > 1) {
-              const float q1 = __shfl_sync(mask, f[NV - 1][e], pl, LPR);
-              q = pi ? q1 : q;
-            }
-            o[i][e] = q;
+          for (int q = 0; q < 4; ++q) {
+            w[q] = __shfl_sync(mask, reinterpret_cast<const uint32_t *>(&raw[0])[q], pl, LPR);
+            const uint32_t w1 = __shfl_sync(mask, reinterpret_cast<const uint32_t *>(&raw[NV - 1])[q], pl, LPR);
+            w[q] = pi ? w1 : w[q];
           }
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int v = lane + i * LPR;
-          if (v < 2 * hv) {
-            const bool first = v < hv;
-            const int p0 = (first ? v : v - hv) * E;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-              const float2 c = cs[p0 + e];
-              f[i][e] = first ? f[i][e] * c.x - o[i][e] * c.y : f[i][e] * c.x + o[i][e] * c.y;
-            }
-          }
+          Vec16<T> x;
+          x.raw = *reinterpret_cast<const Raw *>(w);
+          x.unpack(o[i]);
         }
       }
-    }
-    T *dst = dst_row<T>(s, p, t0 + t, slot, h);
-    if (dst) {
+      request(n + 1);
+      float rstd = 1.0f;
+      if (norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < E; ++e) ss = fmaf(f[i][e], f[i][e], ss);
+#pragma unroll
+        for (int k = LPR / 2; k > 0; k >>= 1) ss += __shfl_xor_sync(mask, ss, k);
+        rstd = rsqrtf(fmaf(ss, inv_d, p.eps));
+      }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int v = lane + i * LPR;
-        if (v < nvec) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float y = f[i][e] * A[i][e];
+          // elements that are not rotated have no partner
+          f[i][e] = rstd * (rotate && v < rotv ? fmaf(o[i][e], B[i][e], y) : y);
+        }
+        if (dst && v < nvec) {
           Vec16<T> x;
           x.pack(f[i]);
-          st_stream_as<Raw>(dst + v * E, x.raw);
+          st_stream_as<Raw>(dst + i * LPR * E, x.raw);
         }
       }
     }
+    dst += dst_step;
   }
   pdl_launch_dependents();
 }
@@ -235,7 +284,7 @@ head_rows_kernel(const Params p, const __grid_constant__ Freqs fr) {
 // the output may be the input here too.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
-head_rows_scalar_kernel(const Params p, const __grid_constant__ Freqs fr) {
+head_rows_scalar_kernel(const Params p) {
   const int lane = threadIdx.x & 31;
   const int heads = p.seg[0].heads + p.seg[1].heads;
   const int64_t rows = p.tokens * heads, step = (int64_t)gridDim.x * (THREADS / 32);
@@ -264,7 +313,7 @@ head_rows_scalar_kernel(const Params p, const __grid_constant__ Freqs fr) {
     auto at = [&](int d) { return to_f32<T>(src[d]) * (w ? rstd * to_f32<T>(w[d]) : rstd); };
     for (int pr = lane; pr < nrot; pr += 32) {
       const int i = p.interleaved ? 2 * pr : pr, j = p.interleaved ? 2 * pr + 1 : pr + half;
-      const float2 c = turn(p.positions[t], fr.turns[pr]);
+      const float2 c = turn(p.positions[t], frequency(p, pr));
       const float a = at(i), b = at(j);
       dst[i] = from_f32<T>(a * c.x - b * c.y);
       dst[j] = from_f32<T>(a * c.y + b * c.x);
@@ -274,24 +323,10 @@ head_rows_scalar_kernel(const Params p, const __grid_constant__ Freqs fr) {
   pdl_launch_dependents();
 }
 
-// Frequencies in turns; the table of the last (theta, rotary_dim) is kept per host thread.
-static const Freqs &freqs(float theta, int rot) {
-  static thread_local Freqs f;
-  static thread_local float f_theta = 0.f;
-  static thread_local int f_rot = -1;
-  if (f_rot != rot || f_theta != theta) {
-    for (int i = 0; i < kMaxPairs; ++i)
-      f.turns[i] = i < rot / 2 ? pow((double)theta, -2.0 * i / rot) / 6.283185307179586476925 : 0.0;
-    f_rot = rot;
-    f_theta = theta;
-  }
-  return f;
-}
-
 template <typename T>
 static bool vector_ok(const Params &p) {
   constexpr int E = Vec16<T>::N;
-  if (p.D % E || p.D > 256 || (!p.interleaved && p.rot % (2 * E))) return false;
+  if (p.D % E || p.D > 256 || p.rot % (p.interleaved ? E : 2 * E)) return false;
   for (const Segment &s : p.seg) {
     if (!s.heads) continue;
     if (!aligned16(s.src) || !aligned16(s.dst) || (s.weight && !aligned16(s.weight))) return false;
@@ -301,45 +336,42 @@ static bool vector_ok(const Params &p) {
 }
 
 template <typename T, int LPR, int NV>
-static cudaError_t launch_vec(const Params &p, const Freqs &fr, dim3 grid, size_t smem, cudaStream_t st) {
-  return launch_pdl(head_rows_kernel<T, LPR, NV>, grid, dim3(THREADS), smem, st, p, fr);
+static cudaError_t launch_vec(const Params &p, dim3 grid, size_t smem, cudaStream_t st) {
+  return launch_pdl(head_rows_kernel<T, LPR, NV>, grid, dim3(THREADS), smem, st, p);
 }
 
 template <typename T>
 static int launch(Params p, float theta, cudaStream_t st) {
   DeviceInfo di;
   if (int e = current_device(&di)) return e;
-  const Freqs &fr = freqs(theta, p.rot);
-  const int heads = p.seg[0].heads + p.seg[1].heads;
+  for (int b = 0; b < kPowerBits && (p.rot >> (b + 1)); ++b) {
+    const double v = ldexp(pow((double)theta, -ldexp(2.0, b) / p.rot), 63);
+    p.power[b] = v < 9223372036854775808.0 ? (uint64_t)v : 1ull << 63;
+  }
   if (!vector_ok<T>(p)) {
-    const int64_t warps = p.tokens * heads, want = (warps + 7) / 8, cap = (int64_t)di.sm_count * 32;
-    HEXB_CUDA_OK(launch_pdl(head_rows_scalar_kernel<T>, dim3((unsigned)(want < cap ? want : cap)), dim3(THREADS), 0, st, p, fr));
+    const int64_t warps = p.tokens * (p.seg[0].heads + p.seg[1].heads), want = (warps + 7) / 8, cap = (int64_t)di.sm_count * 32;
+    HEXB_CUDA_OK(launch_pdl(head_rows_scalar_kernel<T>, dim3((unsigned)(want < cap ? want : cap)), dim3(THREADS), 0, st, p));
     return check_launch("head_rows_scalar");
   }
   constexpr int E = Vec16<T>::N;
   const int nvec = p.D / E;
-  const int lpr = nvec <= 8 ? 8 : nvec <= 16 ? 16 : 32;
+  const int lpr = nvec <= 8 ? 4 : nvec <= 16 ? 8 : nvec <= 32 ? 16 : 32;   // two vectors a lane
   const int rp = THREADS / lpr;
-  // Enough tokens per CTA for four rounds of rows, so that the angles are shared by many rows; a step with few
-  // tokens is cut over its rows instead, one round per CTA.
-  int tb = 4 * rp / heads;
-  const int64_t spread = p.tokens / ((int64_t)di.sm_count * 4);
-  if (tb > spread) tb = (int)spread;
-  if (tb > 16) tb = 16;
-  if (tb < 1) tb = 1;
+  // Tokens per CTA: so many that a group of lanes gets four of a token's heads, but no fewer CTAs than two an SM.
+  int tb = 1;
+  while (tb < rp && rp / tb * 4 > p.seg[0].heads) tb *= 2;
+  while (tb > 1 && (p.tokens + tb - 1) / tb < 2 * (int64_t)di.sm_count) tb /= 2;
   p.tokens_per_cta = tb;
-  int splits = 1;
-  if (tb == 1 && p.tokens < di.sm_count * 4) splits = (heads + rp - 1) / rp;
-  p.rows_per_split = (tb * heads + splits - 1) / splits;
+  for (p.gpt_shift = 0; (tb << (p.gpt_shift + 1)) <= rp;) ++p.gpt_shift;
   const int64_t gx = (p.tokens + tb - 1) / tb;
-  if (gx > 0x7fffffff || splits > 65535) return HEXB_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)gx, (unsigned)splits);
+  if (gx > 0x7fffffff) return HEXB_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)gx);
   const size_t smem = (size_t)tb * (p.rot / 2) * sizeof(float2);
   cudaError_t e;
-  if (lpr == 8) e = launch_vec<T, 8, 1>(p, fr, grid, smem, st);
-  else if (lpr == 16) e = launch_vec<T, 16, 1>(p, fr, grid, smem, st);
-  else if (nvec <= 32) e = launch_vec<T, 32, 1>(p, fr, grid, smem, st);
-  else e = launch_vec<T, 32, 2>(p, fr, grid, smem, st);
+  if (lpr == 4) e = launch_vec<T, 4, 2>(p, grid, smem, st);
+  else if (lpr == 8) e = launch_vec<T, 8, 2>(p, grid, smem, st);
+  else if (lpr == 16) e = launch_vec<T, 16, 2>(p, grid, smem, st);
+  else e = launch_vec<T, 32, 2>(p, grid, smem, st);
   HEXB_CUDA_OK(e);
   return check_launch("head_rows");
 }
@@ -372,9 +404,9 @@ extern "C" int hexb_qk_norm_rope(int dtype, const void *q, const void *k, void *
     return HEXB_ERR_BAD_ARG;
   if (tokens == 0 || D == 0 || q_heads + kv_heads == 0) return HEXB_OK;
   if (!strides || (q_heads && (!q || !q_out)) || (kv_heads && (!k || !k_out)) || (rotary_dim && !positions) ||
-      !(theta > 0.f))
+      !(theta >= 1.f))
     return HEXB_ERR_BAD_ARG;
-  if (D > 4096 || rotary_dim > 2 * heads::kMaxPairs || q_heads + kv_heads > 65535) return HEXB_ERR_UNSUPPORTED;
+  if (D > 4096 || q_heads + kv_heads > 65535) return HEXB_ERR_UNSUPPORTED;
   heads::Params p = {};
   p.seg[0] = {q, q_out, q_weight, strides[0], strides[1], strides[4], strides[5], 0, (int)q_heads, 1, rotary_dim > 0};
   p.seg[1] = {k, k_out, k_weight, strides[2], strides[3], strides[6], strides[7], 0, (int)kv_heads, 1, rotary_dim > 0};
@@ -397,10 +429,10 @@ extern "C" int hexb_kv_cache_append(int dtype, const void *k, const void *v, voi
       rotary_dim % 2)
     return HEXB_ERR_BAD_ARG;
   if (tokens == 0 || kv_heads == 0 || D == 0) return HEXB_OK;
-  if (!strides || !k || !v || !k_cache || !v_cache || !slots || (rotary_dim && !positions) || !(theta > 0.f) ||
+  if (!strides || !k || !v || !k_cache || !v_cache || !slots || (rotary_dim && !positions) || !(theta >= 1.f) ||
       page_size == 0)
     return HEXB_ERR_BAD_ARG;
-  if (D > 4096 || rotary_dim > 2 * heads::kMaxPairs || kv_heads > 32767 || page_size > 0x7fffffff ||
+  if (D > 4096 || kv_heads > 32767 || page_size > 0x7fffffff ||
       num_pages > INT64_MAX / page_size) return HEXB_ERR_UNSUPPORTED;
   heads::Params p = {};
   p.seg[0] = {k, k_cache, k_weight, strides[0], strides[1], strides[5], strides[6], strides[4], (int)kv_heads,

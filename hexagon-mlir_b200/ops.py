@@ -565,8 +565,8 @@ def _rotary(what: str, D: int, rotary_dim, theta: float, positions, tokens: int)
     rot = D if rotary_dim is None else int(rotary_dim)
     if positions.dtype != torch.int64 or positions.shape != (tokens,) or not positions.is_contiguous():
         raise ValueError(f"{what}: positions must be a contiguous int64 [tokens] vector")
-    if rot < 0 or rot > D or rot % 2 or not theta > 0:
-        raise ValueError(f"{what}: rotary_dim must be even and at most D, theta positive")
+    if rot < 0 or rot > D or rot % 2 or not theta >= 1:
+        raise ValueError(f"{what}: rotary_dim must be even and at most D, theta at least 1")
     return rot
 
 
