@@ -70,7 +70,10 @@ paged_rows_kernel(const Params p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rw = warp % RW, kw = warp / RW;
   const int h = blockIdx.z;
-  pdl_wait();
+  // The launch over own keys does not read what the prefix launch of the same call writes until it joins them: it may
+  // run beside it (the prefix launch lets it start only when all that came before is complete).
+  if (!OWN || !p.follows_prefix) pdl_wait();
+  if (!OWN) pdl_launch_dependents();
 
   int tok0 = 0, ntok, hi_all, nq = 0, part, lo, hi;
   const int *pages;
@@ -261,6 +264,7 @@ paged_rows_kernel(const Params p) {
       if (j + 3 < blocks) publish(j + 3, page_next);
     }
     cp_async_wait<0>();
+    if (OWN && p.merge) pdl_wait();  // the prefix parts are complete
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
@@ -304,7 +308,7 @@ paged_rows_kernel(const Params p) {
           f[0] = fmaf(a, v.x, f[0]); f[1] = fmaf(a, v.y, f[1]); f[2] = fmaf(a, v.z, f[2]); f[3] = fmaf(a, v.w, f[3]);
         }
         const int t = tok0 + (row0 + r) / p.G, hd = h * p.G + (row0 + r) % p.G;
-        store4(p, part, t, hd, d, f, mm, ll);
+        store_row<4>(p, part, t, hd, d, f, mm, ll);
       }
     } else {
 #pragma unroll
@@ -313,12 +317,16 @@ paged_rows_kernel(const Params p) {
 #pragma unroll
         for (int n = 0; n < DP / 8; ++n) {
           const int d = n * 8 + (lane & 3) * 2;
-          if (d < p.D) store2(p, part, tok[i], head[i], d, o[n][2 * i], o[n][2 * i + 1], m[i], l[i]);
+          float f[2] = {o[n][2 * i], o[n][2 * i + 1]};
+          if (d < p.D) store_row<2>(p, part, tok[i], head[i], d, f, m[i], l[i]);
         }
       }
     }
   }
-  pdl_launch_dependents();
+  if (OWN) {
+    pdl_wait();  // whoever waits for this launch waits for the prefix launch too
+    pdl_launch_dependents();
+  }
 }
 
 // ------------------------------------------------------------------ join of the parts
@@ -356,18 +364,55 @@ static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // How a call is cut.  A function of the sizes alone, so that the workspace query and the launch agree.
 struct Plan {
+  bool seq, tc_prefix;            // tensor-core forms
   int prefix_parts, prefix_chunk, own_parts;
   int prefix_rw, own_rw;
+  int tile_tokens, piece;
+  int parts() const { return prefix_parts + own_parts; }
+  bool merge() const { return prefix_parts > 0 && own_parts == 1; }
 };
 
 static int rw_for(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
 static Plan make_plan(const hexb_paged_attention_desc *d, int sm_count) {
   Plan pl = {};
-  const int64_t G = d->Hq / d->Hkv;
-  const int per_sm = d->D <= 64 ? 4 : d->D <= 128 ? 2 : 1;
-  const int64_t want = (int64_t)sm_count * per_sm * 2;   // two waves: ragged lengths even out
-  if (d->prefix_len > 0) {
+  const int64_t G = d->Hq / d->Hkv, capacity = d->table_width * d->page_size;
+  const int64_t mq = d->max_q > 0 ? d->max_q : ceil_div(d->T, d->B);
+  const int64_t pblocks = ceil_div(d->prefix_len, 64);
+  // The tensor-core forms: what TMA can address (page pieces of at least the 8 rows of a swizzle atom, no stride of 0), a
+  // positive scale, and enough rows to fill half of a 128-row tile; below that the key stream, not the products, is
+  // what takes the time, and the small tiles of mma.sync read it as fast.
+  pl.piece = (int)(d->page_size & -d->page_size);
+  if (pl.piece > 64) pl.piece = 64;
+  bool tc_ok = (d->D == 64 || d->D == 128) && pl.piece >= 8 && d->sm_scale > 0.f && G <= 128;
+  const int64_t dims[10] = {d->T, d->Hq, d->num_pages, d->page_size, d->Hkv, d->num_pages, d->page_size, d->Hkv, 1, 1};
+  for (int i = 0; i < 8; ++i) tc_ok = tc_ok && (dims[i] <= 1 || (d->strides[i] > 0 && d->strides[i] < ((int64_t)1 << 38)));
+  tc_ok = tc_ok && (d->Hkv <= 1 || d->strides[1] * G < ((int64_t)1 << 38));
+  pl.tile_tokens = tc_ok ? (int)(128 / G) : 0;
+  if (tc_ok && mq * G >= 64 && capacity > 0) {
+    // tiles of one sequence each, over prefix and own keys: cut the axis only when the tiles leave SMs idle
+    pl.seq = true;
+    const int64_t tiles = d->B * ceil_div(mq, pl.tile_tokens) * d->Hkv;
+    int64_t parts = 2 * sm_count / tiles;
+    const int64_t most = (pblocks + capacity / 64) / 8;
+    if (parts > most) parts = most;
+    if (parts > 32) parts = 32;
+    pl.prefix_parts = parts > 1 ? (int)parts : 1;
+    return pl;
+  }
+  if (d->prefix_len > 0 && tc_ok && d->T * G >= 64) {
+    // One CTA an SM when own keys follow: their launch shares the SMs and streams beside the products.
+    pl.tc_prefix = true;
+    const int64_t tiles = (int64_t)ceil_div(d->T, pl.tile_tokens) * d->Hkv;
+    int64_t parts = (capacity > 0 ? 1 : 2) * sm_count / tiles;
+    if (parts < 1) parts = 1;
+    if (parts > 64) parts = 64;
+    if (parts > (pblocks + 1) / 2) parts = (pblocks + 1) / 2;
+    const int64_t per = ceil_div(pblocks, parts);
+    pl.prefix_parts = ceil_div(pblocks, per);
+  } else if (d->prefix_len > 0) {
+    const int per_sm = d->D <= 64 ? 4 : d->D <= 128 ? 2 : 1;
+    const int64_t want = (int64_t)sm_count * per_sm * 2;
     pl.prefix_rw = rw_for(d->T * G);
     const int64_t tiles = (int64_t)ceil_div(d->T * G, 16 * pl.prefix_rw) * d->Hkv;
     int64_t parts = ceil_div(want, tiles);
@@ -377,25 +422,22 @@ static Plan make_plan(const hexb_paged_attention_desc *d, int sm_count) {
     pl.prefix_chunk = ceil_div(ceil_div(d->prefix_len, parts), 64) * 64;
     pl.prefix_parts = ceil_div(d->prefix_len, pl.prefix_chunk);
   }
-  const int64_t capacity = d->table_width * d->page_size;
   if (capacity > 0) {
-    const int64_t mq = d->max_q > 0 ? d->max_q : ceil_div(d->T, d->B);
     pl.own_rw = rw_for(mq * G);
     const int64_t tiles = (int64_t)d->B * ceil_div(mq * G, 16 * pl.own_rw) * d->Hkv;
-    int64_t parts = ceil_div(want, tiles);
+    int64_t parts = sm_count * 2 / tiles;   // one part (and no join launch) once the tiles fill the SMs
     const int64_t most = ceil_div(capacity, 256);
     if (parts > most) parts = most;
     if (parts > 64) parts = 64;
-    pl.own_parts = (int)parts;
+    pl.own_parts = parts > 1 ? (int)parts : 1;
   }
   return pl;
 }
 
 static size_t ws_need(const hexb_paged_attention_desc *d, const Plan &pl) {
-  const size_t parts = (size_t)pl.prefix_parts + pl.own_parts;
-  if (parts < 2) return 0;
-  const size_t n = (size_t)d->T * d->Hq;
-  return parts * n * ((size_t)d->D * 4 + 8) + 256;
+  if (pl.parts() < 2) return 0;
+  const size_t parts = pl.merge() ? (size_t)pl.prefix_parts : (size_t)pl.parts();
+  return parts * (size_t)d->T * d->Hq * ((size_t)d->D * 4 + 8) + 256;
 }
 
 template <int DP, int RW, bool OWN>
@@ -485,26 +527,41 @@ extern "C" int hexb_paged_attention_f16(const hexb_paged_attention_desc *d, void
   p.own_capacity = (int)(d->table_width * d->page_size);
   p.prefix_parts = pl.prefix_parts; p.prefix_chunk = pl.prefix_chunk; p.own_parts = pl.own_parts;
   p.scale_log2 = d->sm_scale * 1.44269504f;
+  p.tile_tokens = pl.tile_tokens;
+  p.piece = pl.piece;
   if (need) {
-    const size_t n = (size_t)(pl.prefix_parts + pl.own_parts) * d->T * d->Hq;
+    const size_t n = (size_t)(pl.merge() ? pl.prefix_parts : pl.parts()) * d->T * d->Hq;
     uint8_t *w = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~(uintptr_t)15);
     p.part_o = reinterpret_cast<float *>(w);
     p.part_ml = reinterpret_cast<float2 *>(w + n * d->D * 4);
   }
   cudaStream_t st = (cudaStream_t)stream;
-  if (pl.prefix_parts) {
-    const int64_t rows = d->T * p.G, tile = 16 * pl.prefix_rw;
-    const dim3 grid((unsigned)((rows + tile - 1) / tile), (unsigned)pl.prefix_parts, (unsigned)d->Hkv);
+  const int64_t mq = d->max_q > 0 ? d->max_q : paged::ceil_div(d->T, d->B);
+  auto grid_of = [&](int64_t x, int64_t y, dim3 *g) {
+    if (x > 0x7fffffff || y > 65535) return false;
+    *g = dim3((unsigned)x, (unsigned)y, (unsigned)d->Hkv);
+    return true;
+  };
+  dim3 grid;
+  if (pl.seq) {
+    if (!grid_of(paged::ceil_div(mq, pl.tile_tokens), (int64_t)pl.prefix_parts * d->B, &grid)) return HEXB_ERR_UNSUPPORTED;
+    if (int e = paged::tc_launch(p, (int)d->Hkv, true, grid, st)) return e;
+  } else if (pl.tc_prefix) {
+    if (!grid_of(paged::ceil_div(d->T, pl.tile_tokens), pl.prefix_parts, &grid)) return HEXB_ERR_UNSUPPORTED;
+    if (int e = paged::tc_launch(p, (int)d->Hkv, false, grid, st)) return e;
+  } else if (pl.prefix_parts) {
+    if (!grid_of(paged::ceil_div(d->T * p.G, 16 * pl.prefix_rw), pl.prefix_parts, &grid)) return HEXB_ERR_UNSUPPORTED;
     if (int e = paged::dispatch_rows<false>(p, pl.prefix_rw, grid, st)) return e;
   }
   if (pl.own_parts) {
-    const int64_t mq = d->max_q > 0 ? d->max_q : paged::ceil_div(d->T, d->B);
-    const int64_t tile = 16 * pl.own_rw, ny = (int64_t)pl.own_parts * d->B;
-    if (ny > 65535) return HEXB_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)((mq * p.G + tile - 1) / tile), (unsigned)ny, (unsigned)d->Hkv);
-    if (int e = paged::dispatch_rows<true>(p, pl.own_rw, grid, st)) return e;
+    if (!grid_of(paged::ceil_div(mq * p.G, 16 * pl.own_rw), (int64_t)pl.own_parts * d->B, &grid)) return HEXB_ERR_UNSUPPORTED;
+    paged::Params po = p;
+    po.follows_prefix = pl.prefix_parts > 0;
+    po.merge = pl.merge();
+    if (int e = paged::dispatch_rows<true>(po, pl.own_rw, grid, st)) return e;
+    if (pl.merge()) return HEXB_OK;
   }
-  if (pl.prefix_parts + pl.own_parts != 1) {
+  if (pl.parts() != 1) {
     // also the call without any key: its rows are set to zero
     const int64_t rows = d->T * d->Hq;
     HEXB_CUDA_OK(launch_pdl(paged::paged_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p));

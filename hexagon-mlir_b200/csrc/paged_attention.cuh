@@ -23,6 +23,9 @@ struct Params {
   float scale_log2;
   float *part_o;                      // [part][T * Hq][D]
   float2 *part_ml;                    // [part][T * Hq]: row maximum (base 2) and sum
+  int tile_tokens, piece;             // tensor-core form: tokens of a tile, keys of one TMA box
+  int follows_prefix;                 // this launch may start while the call's prefix launch is still running
+  int merge;                          // and joins its parts with its own result instead of storing a part
 };
 
 // Tokens [tok0, tok0 + n) of sequence b.  Offsets are data on the device: whatever they hold, the rows
@@ -46,30 +49,68 @@ __device__ __forceinline__ int seq_len(const Params &p, int b) {
   return min(max(n, 0), p.own_capacity);
 }
 
-// Results of a part, or the output itself when the call has one part.  l == 0 marks a part in which the row saw
-// no key: its O is neither stored nor read.
-__device__ __forceinline__ void store4(const Params &p, int part, int t, int hd, int d, const float (&f)[4], float m, float l) {
-  if (p.part_o) {
+// out = join of the prefix parts and (f, m, l), elements d .. d + W - 1 of one row.
+template <int W>
+__device__ __forceinline__ void merge_row(const Params &p, int t, int hd, int d, float (&f)[W], float m, float l) {
+  const int64_t n = (int64_t)p.T * p.Hq, row = (int64_t)t * p.Hq + hd;
+  float mm = l == 0.f ? -INFINITY : m;
+  for (int i = 0; i < p.prefix_parts; ++i) {
+    const float2 ml = __ldcg(&p.part_ml[i * n + row]);
+    if (ml.y != 0.f) mm = fmaxf(mm, ml.x);
+  }
+  const float a = l == 0.f ? 0.f : exp2f(m - mm);
+  float ll = l * a;
+#pragma unroll
+  for (int e = 0; e < W; ++e) f[e] = l == 0.f ? 0.f : f[e] * a;
+#pragma unroll 4
+  for (int i = 0; i < p.prefix_parts; ++i) {
+    const float2 ml = __ldcg(&p.part_ml[i * n + row]);
+    if (ml.y == 0.f) continue;
+    const float w = exp2f(ml.x - mm);
+    ll = fmaf(w, ml.y, ll);
+    const float *o = p.part_o + (i * n + row) * p.D + d;
+    float v[W];
+    if (W == 4) {
+      const float4 q = __ldcg(reinterpret_cast<const float4 *>(o));
+      v[0] = q.x; v[1] = q.y; v[W - 2] = q.z; v[W - 1] = q.w;
+    } else {
+      const float2 q = __ldcg(reinterpret_cast<const float2 *>(o));
+      v[0] = q.x; v[1] = q.y;
+    }
+#pragma unroll
+    for (int e = 0; e < W; ++e) f[e] = fmaf(w, v[e], f[e]);
+  }
+  const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+  __half2 *o = reinterpret_cast<__half2 *>(p.out + (int64_t)t * p.so_t + (int64_t)hd * p.so_h + d);
+#pragma unroll
+  for (int e = 0; e < W; e += 2) o[e / 2] = __floats2half2_rn(f[e] * inv, f[e + 1] * inv);
+}
+
+// Result of a part, elements d .. d + W - 1 of one row, or the output itself when the call has one part.  l == 0 marks a
+// part in which the row saw no key: its O is neither stored nor read.
+template <int W>
+__device__ __forceinline__ void store_row(const Params &p, int part, int t, int hd, int d, float (&f)[W], float m, float l) {
+  if (p.merge) {
+    merge_row<W>(p, t, hd, d, f, m, l);
+  } else if (p.part_o) {
     const int64_t i = (int64_t)part * p.T * p.Hq + (int64_t)t * p.Hq + hd;
     if (d == 0) p.part_ml[i] = make_float2(m, l);
-    if (l != 0.f) *reinterpret_cast<float4 *>(p.part_o + i * p.D + d) = make_float4(f[0], f[1], f[2], f[3]);
+    if (l != 0.f) {
+      float2 *o = reinterpret_cast<float2 *>(p.part_o + i * p.D + d);
+      if (W == 4) *reinterpret_cast<float4 *>(o) = make_float4(f[0], f[1], f[W - 2], f[W - 1]);
+      else *o = make_float2(f[0], f[1]);
+    }
   } else {
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     __half2 *o = reinterpret_cast<__half2 *>(p.out + (int64_t)t * p.so_t + (int64_t)hd * p.so_h + d);
-    o[0] = __floats2half2_rn(f[0] * inv, f[1] * inv);
-    o[1] = __floats2half2_rn(f[2] * inv, f[3] * inv);
+#pragma unroll
+    for (int e = 0; e < W; e += 2) o[e / 2] = __floats2half2_rn(f[e] * inv, f[e + 1] * inv);
   }
 }
-__device__ __forceinline__ void store2(const Params &p, int part, int t, int hd, int d, float a, float b, float m, float l) {
-  if (p.part_o) {
-    const int64_t i = (int64_t)part * p.T * p.Hq + (int64_t)t * p.Hq + hd;
-    if (d == 0) p.part_ml[i] = make_float2(m, l);
-    if (l != 0.f) *reinterpret_cast<float2 *>(p.part_o + i * p.D + d) = make_float2(a, b);
-  } else {
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    *reinterpret_cast<__half2 *>(p.out + (int64_t)t * p.so_t + (int64_t)hd * p.so_h + d) = __floats2half2_rn(a * inv, b * inv);
-  }
-}
+
+// Tensor-core form (paged_attention_tc.cu): seq false: rows of the batch against the prefix; true: rows of each
+// sequence against the prefix and its own keys.
+int tc_launch(const Params &p, int hkv, bool seq, dim3 grid, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace hexb

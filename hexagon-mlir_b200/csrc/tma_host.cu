@@ -263,6 +263,7 @@ int softmax_device_status_fetch_and_clear(int *out);
 int embed_device_status_fetch_and_clear(int *out);
 int heads_device_status_fetch_and_clear(int *out);
 int paged_device_status_fetch_and_clear(int *out);
+int paged_tc_device_status_fetch_and_clear(int *out);
 
 }  // namespace hexb
 
@@ -270,7 +271,7 @@ extern "C" int hexb_device_status(int *out) {
   using namespace hexb;
   if (!out) return HEXB_ERR_BAD_ARG;
   HEXB_CUDA_OK(cudaDeviceSynchronize());
-  int v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  int v[9] = {};
   if (int s = gemm_device_status_fetch_and_clear(&v[0])) return s;
   if (int s = attn_device_status_fetch_and_clear(&v[1])) return s;
   if (int s = norm_device_status_fetch_and_clear(&v[2])) return s;
@@ -279,8 +280,9 @@ extern "C" int hexb_device_status(int *out) {
   if (int s = selftest_device_status_fetch_and_clear(&v[5])) return s;
   if (int s = heads_device_status_fetch_and_clear(&v[6])) return s;
   if (int s = paged_device_status_fetch_and_clear(&v[7])) return s;
+  if (int s = paged_tc_device_status_fetch_and_clear(&v[8])) return s;
   *out = 0;
-  for (int i = 7; i >= 0; --i)
+  for (int i = 8; i >= 0; --i)
     if (v[i]) *out = v[i];
   return HEXB_OK;
 }

@@ -278,8 +278,8 @@ int hexb_decoder_forward_f16_noalloc(const hexb_decoder_config *cfg, const hexb_
  *   out[t, h, :] = R(positions[t]) . (x[t, h, :] * rsqrt(mean(x[t, h, :]^2) + eps) * weight)
  * q, q_out [tokens, q_heads, D] and k, k_out [tokens, kv_heads, D]; strides[8] = (token, head) of q, k, q_out,
  * k_out in elements (innermost 1).  q_weight / k_weight [D], NULL for ones.  R turns the pairs of the first
- * rotary_dim elements (even, <= D and <= 512; 0: no rotation, positions may be NULL) by position *
- * theta^(-2p / rotary_dim): pair (2p, 2p+1) when interleaved != 0 (the convention of hexb_rope), else
+ * rotary_dim elements (even, <= D; 0: no rotation, positions may be NULL) by position *
+ * theta^(-2p / rotary_dim), theta >= 1: pair (2p, 2p+1) when interleaved != 0 (the convention of hexb_rope), else
  * (p, p + rotary_dim/2).  q_out may be q, and k_out k (same strides); other overlaps are not allowed. D <= 4096. */
 int hexb_qk_norm_rope(int dtype, const void *q, const void *k, void *q_out, void *k_out, const int64_t *positions,
                       const void *q_weight, const void *k_weight, int64_t tokens, int64_t q_heads, int64_t kv_heads,

@@ -18,7 +18,7 @@ def test_qk_norm_rope_status_codes():
     assert call(dt=6) == -2 and call(T=-1) == -1 and call(rot=66) == -1 and call(rot=3) == -1
     assert call(T=0) == 0 and call(D=0, rot=0) == 0 and call(Hq=0, Hkv=0) == 0
     assert call(ptr=None) == -1 and call(pos=None) == -1 and call(theta=0.0) == -1 and call(theta=float("nan")) == -1
-    assert call(D=5000, rot=0) == -2 and call(D=1024, rot=514) == -2
+    assert call(D=5000, rot=0) == -2 and call(Hq=65000, Hkv=1000) == -2
 
 
 def test_kv_cache_append_status_codes():
@@ -57,8 +57,8 @@ def test_paged_attention_status_codes():
         assert call(**bad) == -2, bad
     assert call(Q=4104) == -3 and call(V_cache=4098) == -3 and call(strides=(i64 * 10)(*([4] * 10))) == -3
     assert call(T=0, B=0) == 0 and call(Hq=0) == 0
-    # one query row per CTA at least, two parts (prefix and own keys): a workspace is needed, the query says so
-    assert lib.hexb_paged_attention_workspace_bytes(C.byref(desc())) >= 2 * 4 * 8 * (64 * 4 + 8)
+    # the prefix and the own keys are computed apart and joined: a workspace is needed, the query says so
+    assert lib.hexb_paged_attention_workspace_bytes(C.byref(desc())) >= 4 * 8 * (64 * 4 + 8)
     assert lib.hexb_paged_attention_workspace_bytes(C.byref(desc(T=0, B=0))) == 0
     assert lib.hexb_paged_attention_workspace_bytes(C.byref(desc(D=60))) == 0
 
