@@ -12,6 +12,9 @@
 // A row that sees no key (empty sequence, no prefix) gives zeros.  Rows behind the last sequence are not
 // written.  fp32 scores, statistics and sums; P is rounded to fp16 for the second product as in the library's
 // other attention kernels, and the output once.
+#include <type_traits>
+
+#include "attn_common.cuh"
 #include "paged_attention.cuh"
 
 namespace hexb {
@@ -42,193 +45,253 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// ------------------------------------------------------------------ tiles of few rows
-// One CTA: a tile of 16 * RW rows of one key head against a range of keys, in blocks of 64 keys staged by
-// cp.async through a three-deep ring.  RW row groups times 4 / RW key groups of warps: with few rows (a decode
-// step) the four warps share the rows and take 16 keys of a block each, with their own running maximum and sum,
-// joined at the end; with many rows each warp owns 16 rows and all keys.
-// OWN false: rows of the whole batch against the shared prefix (split blockIdx.y of it).
-// OWN true: rows of sequence blockIdx.y % B against its own keys, split blockIdx.y / B.
+// ------------------------------------------------------------------ stream of key blocks
+// Tiles of 16 * RW rows of one key head against blocks of 64 keys, four consumer warps.  RW row groups times 4 / RW key
+// groups of warps: with few rows (a decode step) the four warps share the rows and take 16 keys of a block each,
+// with their own running maximum and sum, joined at the end of a run; with many rows each warp owns 16 rows and all
+// keys.
+//
+// The work of a call is one list of units -- (sequence, key head, tile, block), the shared prefix counting as a
+// sequence of all tokens -- cut evenly over the CTAs that fit the GPU.  A CTA streams its stretch of the list without a
+// pause at the borders between sequences: the start-up (lengths, page numbers, first keys: three dependent trips
+// to memory) is paid once, and ragged lengths leave no SM idle.  A run of units of one tile ends in one part; the
+// join adds the parts up.
+//
+// The stream is bound by memory only if a block costs its warps few instructions: with every thread copying its share
+// by cp.async (page, address and predicate for each 16 bytes) a block cost 550 instructions a warp and the stream
+// ran at 4.9 TB/s of 8192-key sequences.  So a producer warp fetches blocks by TMA, page piece by page
+// piece, the consumer warps wait on its barriers and not on each other, and O is rescaled only when a row maximum grows by
+// more than 2^8.  The cp.async form remains for pages and strides that TMA cannot address.
 template <int DP>
 struct RowCfg {
   static constexpr int BN = 64;
   static constexpr int STAGES = 3;
-  static constexpr int KV = BN * DP * 2;
-  static constexpr int OFFS = STAGES * 2 * KV;           // two buffers of row offsets, K and V
+  static constexpr int KV = BN * DP * 2, KV_CHUNK = BN * 128;   // 64 columns: 64 rows of 128 bytes, 128-byte swizzle
+  // Exchange between the key groups: m, l, and 16 rows of DP / 4 columns a warp.  Heads of more than 128 leave no room
+  // for it beside three stages: their tiles have 64 rows, a warp owns all keys of its 16.
+  static constexpr int XCH = STAGES * 2 * KV;
+  static constexpr int OFFS = XCH + (DP > 128 ? 0 : (128 + 64 * (DP / 4 + 2)) * 4);   // cp.async: row offsets, K and V, two buffers
+  static constexpr int BARS = OFFS;                      // TMA: full and empty barrier of every stage, abort flag
   static constexpr int SMEM = OFFS + 2 * 2 * BN * 8;
+  static constexpr int SMEM_TMA = BARS + 2 * STAGES * 8 + 16 + 1024;
+  static constexpr int PER_SM = DP == 64 ? 4 : DP == 128 ? 2 : 1;
 };
 
-template <int DP, int RW, bool OWN>
-__global__ void __launch_bounds__(THREADS, DP == 64 ? 4 : DP == 128 ? 2 : 1)
-paged_rows_kernel(const Params p) {
-  using cfg = RowCfg<DP>;
-  constexpr int BN = cfg::BN, KW = 4 / RW, KPW = BN / KW, ROWS = 16 * RW;
-  constexpr int CH = DP / 8;  // 16-byte chunks of a row
-  extern __shared__ __align__(128) uint8_t smem[];
-  const uint32_t s0 = (uint32_t)__cvta_generic_to_shared(smem);
-  int64_t *offs = reinterpret_cast<int64_t *>(smem + cfg::OFFS);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rw = warp % RW, kw = warp / RW;
-  const int h = blockIdx.z;
-  // The launch over own keys does not read what the prefix launch of the same call writes until it joins them: it may
-  // run beside it (the prefix launch lets it start only when all that came before is complete).
-  if (!OWN || !p.follows_prefix) pdl_wait();
-  if (!OWN) pdl_launch_dependents();
+// A place in the list of units.
+struct Cursor {
+  int b;                 // -1: the prefix
+  int tok0, ntok, len, nb, nt;
+  int h, tile, j;
+};
 
-  int tok0 = 0, ntok, hi_all, nq = 0, part, lo, hi;
-  const int *pages;
-  if (OWN) {
-    const int b = blockIdx.y % p.B, split = blockIdx.y / p.B;
-    seq_range(p, b, tok0, ntok);
-    nq = ntok;
-    hi_all = seq_len(p, b);
-    pages = p.table + (int64_t)b * p.table_stride;
-    part = p.prefix_parts + split;
-    const int chunk = ((hi_all + p.own_parts - 1) / p.own_parts + BN - 1) / BN * BN;
-    lo = min(split * chunk, hi_all);
-    hi = min(lo + chunk, hi_all);
+template <int RW>
+__device__ __forceinline__ long long sequence_units(const Params &p, int b, int *tok0, int *ntok, int *len) {
+  if (b < 0) {
+    *tok0 = 0;
+    *ntok = tokens_used(p);
+    *len = p.prefix_len;
   } else {
-    ntok = tokens_used(p);
-    hi_all = p.prefix_len;
-    pages = p.prefix_pages;
-    part = blockIdx.y;
-    lo = min(part * p.prefix_chunk, hi_all);
-    hi = min(lo + p.prefix_chunk, hi_all);
+    seq_range(p, b, *tok0, *ntok);
+    *len = seq_len(p, b);
   }
-  const int rows = ntok * p.G;
+  // a tile without keys is one unit too: its rows get an empty part
+  return (long long)((*ntok * p.G + 16 * RW - 1) / (16 * RW)) * (p.Hq / p.G) * max((*len + 63) / 64, 1);
+}
 
-  for (int row0 = (int)blockIdx.x * ROWS; row0 < rows; row0 += (int)gridDim.x * ROWS) {
-    // the last key any row of the tile sees
-    int end = hi;
-    if (OWN) end = min(end, hi_all - nq + min(ntok - 1, (row0 + ROWS - 1) / p.G) + 1);
-    const int blocks = end > lo ? (end - lo + BN - 1) / BN : 0;
+template <int RW>
+__device__ __forceinline__ void enter(const Params &p, Cursor &c) {
+  // the next sequence from c.b on that has tokens
+  for (; c.b < p.nseq; ++c.b) {
+    if (sequence_units<RW>(p, c.b, &c.tok0, &c.ntok, &c.len) > 0) break;
+  }
+  c.nb = max((c.len + 63) / 64, 1);
+  c.nt = (c.ntok * p.G + 16 * RW - 1) / (16 * RW);
+}
 
-    // A fragments of Q: rows g and g + 8 of this warp's 16
-    int tok[2], head[2];
-    bool row_ok[2];
+template <int RW>
+__device__ __forceinline__ void advance(const Params &p, Cursor &c) {
+  if (++c.j < c.nb) return;
+  c.j = 0;
+  if (++c.tile < c.nt) return;
+  c.tile = 0;
+  if (++c.h < p.Hq / p.G) return;
+  c.h = 0;
+  ++c.b;
+  enter<RW>(p, c);
+}
+
+// Keys [0, end) of the cursor's sequence are seen by some row of its tile.
+template <int RW>
+__device__ __forceinline__ int end_of(const Params &p, const Cursor &c) {
+  if (c.b < 0) return c.len;
+  return min(c.len, c.len - c.ntok + min(c.ntok - 1, (c.tile * 16 * RW + 16 * RW - 1) / p.G) + 1);
+}
+
+// This CTA's stretch of the list: units [start, stop), `per` units a CTA, the cursor at start.  All NT threads call it.
+template <int RW, int NT>
+__device__ __forceinline__ void find_stretch(const Params &p, long long &start, long long &stop, long long &per, Cursor &c) {
+  constexpr int NW = NT / 32;
+  __shared__ long long s_sum[NW];
+  __shared__ int s_max[NW];
+  __shared__ int s_b;
+  __shared__ long long s_off;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int first_b = p.stream_prefix ? -1 : 0;
+  long long total = 0;
+  int longest = 0;
+  for (int b = first_b + tid; b < p.nseq; b += NT) {
+    int t0, n, len;
+    const long long u = sequence_units<RW>(p, b, &t0, &n, &len);
+    total += u;
+    // blocks that one part slot has to cover at least, so that a tile's runs fit its slots
+    const int slots = (b < 0 ? p.prefix_parts : p.own_parts) - 1;
+    if (u) longest = max(longest, slots > 0 ? ((len + 63) / 64 + slots - 1) / slots : (len + 63) / 64);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+  }
+  if (lane == 0) {
+    s_sum[warp] = total;
+    s_max[warp] = longest;
+  }
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < NW; ++w) {
+    total += s_sum[w];
+    longest = max(longest, s_max[w]);
+  }
+  per = max((total + gridDim.x - 1) / gridDim.x, (long long)max(longest, 1));
+  start = blockIdx.x * per;
+  stop = min(start + per, total);
+  if (start >= stop) return;
+  long long base = 0;
+  for (int b0 = first_b; b0 < p.nseq; b0 += NT) {
+    int t0, n, len;
+    const long long u = b0 + tid < p.nseq ? sequence_units<RW>(p, b0 + tid, &t0, &n, &len) : 0;
+    long long incl = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    __syncthreads();
+    if (lane == 31) s_sum[warp] = incl;
+    if (tid == 0) s_b = p.nseq;
+    __syncthreads();
+    long long excl = base + incl - u;
+    for (int w = 0; w < warp; ++w) excl += s_sum[w];
+    if (start >= excl && start < excl + u) {
+      s_b = b0 + tid;
+      s_off = start - excl;
+    }
+    for (int w = 0; w < NW; ++w) base += s_sum[w];
+    __syncthreads();
+    if (s_b < p.nseq) break;
+  }
+  c.b = s_b;
+  enter<RW>(p, c);
+  const int off = (int)(s_off % ((long long)c.nb * c.nt)), tile_head = off / c.nb;
+  c.h = (int)(s_off / ((long long)c.nb * c.nt));
+  c.j = off - tile_head * c.nb;
+  c.tile = tile_head;
+}
+
+// The running state of one tile in the consumer warps.
+template <int DP, int RW>
+struct Run {
+  static constexpr int KW = 4 / RW, KPW = 64 / KW, ROWS = 16 * RW;
+  uint32_t qa[DP / 16][4];
+  float o[DP / 8][4];
+  float m[2], l[2];       // reference maximum (base 2, scaled) of rows g and g + 8; this lane's share of the sum
+  int tok[2], head[2];
+  bool row_ok[2];
+  int lane, rw, kw;
+
+  // fragments of Q: rows g and g + 8 of this warp's 16
+  __device__ __forceinline__ void begin(const Params &p, const Cursor &c) {
+    const int row0 = c.tile * ROWS, rows = c.ntok * p.G;
+    const __half *q[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = row0 + rw * 16 + (lane >> 2) + 8 * i;
       row_ok[i] = r < rows;
-      tok[i] = tok0 + (row_ok[i] ? r / p.G : 0);
-      head[i] = h * p.G + (row_ok[i] ? r % p.G : 0);
+      tok[i] = c.tok0 + (row_ok[i] ? r / p.G : 0);
+      head[i] = c.h * p.G + (row_ok[i] ? r % p.G : 0);
+      q[i] = p.q + (int64_t)tok[i] * p.sq_t + (int64_t)head[i] * p.sq_h + (lane & 3) * 2;
+      m[i] = -INFINITY;
+      l[i] = 0.f;
     }
-    uint32_t qa[DP / 16][4];
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int d = k * 16 + (i >> 1) * 8 + (lane & 3) * 2;
+        const int d = k * 16 + (i >> 1) * 8;
         qa[k][i] = 0;
-        if (row_ok[i & 1] && d < p.D)
-          qa[k][i] = *reinterpret_cast<const uint32_t *>(p.q + (int64_t)tok[i & 1] * p.sq_t + (int64_t)head[i & 1] * p.sq_h + d);
+        if (row_ok[i & 1] && d < p.D) qa[k][i] = *reinterpret_cast<const uint32_t *>(q[i & 1] + d);
       }
-
-    // row offsets of block j: thread tid < 64 looks key tid up (one block ahead of its use)
-    auto lookup = [&](int j) -> int {
-      const int key = lo + j * BN + tid;
-      return tid < BN && key < end ? pages[key / p.page_size] : -1;
-    };
-    auto publish = [&](int j, int page) {
-      if (tid < BN) {
-        const int key = lo + j * BN + tid;
-        int64_t ko = -1, vo = -1;
-        if (key < end) {
-          if ((unsigned)page < (unsigned)p.num_pages) {
-            const int64_t in = key % p.page_size;
-            ko = (int64_t)page * p.sk_p + in * p.sk_s;
-            vo = (int64_t)page * p.sv_p + in * p.sv_s;
-          } else {
-            atomicExch(&g_paged_status, (int)HEXB_ERR_BAD_ARG);
-          }
-        }
-        int64_t *o = offs + (j & 1) * 2 * BN;
-        o[tid] = ko;
-        o[BN + tid] = vo;
-      }
-    };
-    auto fetch = [&](int j) {
-      if (j < blocks) {
-        const int64_t *o = offs + (j & 1) * 2 * BN;
-        const uint32_t st = s0 + (uint32_t)(j % cfg::STAGES) * 2 * cfg::KV;
-        const int c = tid % CH;
-        const bool col = c * 8 < p.D;
-#pragma unroll
-        for (int i = 0; i < BN * CH / THREADS; ++i) {
-          const int row = tid / CH + i * (THREADS / CH);
-          const uint32_t dst = st + (uint32_t)(row * DP * 2 + ((c ^ (row & 7)) * 16));
-          const int64_t ko = o[row], vo = o[BN + row];
-          const bool kv = col && ko >= 0;
-          cp_async16(dst, p.k + (kv ? ko + (int64_t)h * p.sk_h + c * 8 : 0), kv);
-          cp_async16(dst + cfg::KV, p.v + (kv ? vo + (int64_t)h * p.sv_h + c * 8 : 0), kv);
-        }
-      }
-      cp_async_commit();
-    };
-
-    float o[DP / 8][4];
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  }
 
-    __syncthreads();  // the previous tile's use of the shared memory is over
-    publish(0, lookup(0));
-    publish(1, lookup(1));
-    __syncthreads();
-    fetch(0);
-    fetch(1);
-    int page_next = lookup(2);
-    __syncthreads();
-    publish(2, page_next);
-    for (int j = 0; j < blocks; ++j) {
-      cp_async_wait<1>();
-      __syncthreads();  // block j landed for all; block j - 1's readers are done; offsets of j + 2 are visible
-      fetch(j + 2);
-      page_next = lookup(j + 3);
-      const uint32_t sk = s0 + (uint32_t)(j % cfg::STAGES) * 2 * cfg::KV, sv = sk + cfg::KV;
-      float s[KPW / 8][4];
+  // One block: keys 64 * c.j .. of the tile, K at sk and V at sv.
+  __device__ __forceinline__ void step(const Params &p, const Cursor &c, int end, uint32_t sk, uint32_t sv) {
+    constexpr int KV_CHUNK = RowCfg<DP>::KV_CHUNK;
+    float s[KPW / 8][4];
 #pragma unroll
-      for (int n = 0; n < KPW / 8; ++n)
+    for (int n = 0; n < KPW / 8; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+    const uint32_t krow = (uint32_t)(kw * KPW + (lane & 7) + ((lane >> 4) << 3)), kx = krow & 7;
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
+    for (int k = 0; k < DP / 16; ++k) {
+      const uint32_t ch = (uint32_t)(k * 2) + ((lane >> 3) & 1);
+      const uint32_t at = sk + (ch >> 3) * KV_CHUNK + krow * 128 + (((ch & 7) ^ kx) << 4);
 #pragma unroll
-        for (int n = 0; n < KPW / 16; ++n) {
-          const int row = kw * KPW + n * 16 + (lane & 7) + ((lane >> 4) << 3);
-          const int c = k * 2 + ((lane >> 3) & 1);
-          uint32_t b[4];
-          ldsm4(sk + (uint32_t)(row * DP * 2 + ((c ^ (row & 7)) * 16)), b);
-          mma16816(s[2 * n], qa[k], b[0], b[1]);
-          mma16816(s[2 * n + 1], qa[k], b[2], b[3]);
-        }
+      for (int n = 0; n < KPW / 16; ++n) {
+        uint32_t b[4];
+        ldsm4(at + n * 16 * 128, b);
+        mma16816(s[2 * n], qa[k], b[0], b[1]);
+        mma16816(s[2 * n + 1], qa[k], b[2], b[3]);
       }
-      // scores in base 2; keys past the end, and for own keys those after the row's token, drop out
-      const int key0 = lo + j * BN + kw * KPW;
-      int limit[2] = {end, end};
-      if (OWN) {
+    }
+    // scores in base 2; keys past the end, and own keys after the row's token, drop out
+    const int key0 = c.j * 64 + kw * KPW;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) limit[i] = min(end, hi_all - nq + (tok[i] - tok0) + 1);
-      }
-      float mx[2] = {m[0], m[1]};
+    for (int n = 0; n < KPW / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] *= p.scale_log2;
+    const int sees = c.b < 0 ? end : c.len - c.ntok + 1 - c.tok0;   // + token: own keys a row sees
+    if (key0 + KPW > (c.b < 0 ? end : c.len - c.ntok + 1)) {        // some row may not see some key of this warp
 #pragma unroll
       for (int n = 0; n < KPW / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int key = key0 + n * 8 + (lane & 3) * 2 + (e & 1);
-          s[n][e] = key < limit[e >> 1] ? s[n][e] * p.scale_log2 : -INFINITY;
-          mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
+          const int limit = min(end, c.b < 0 ? end : sees + tok[e >> 1]);
+          if (key >= limit) s[n][e] = -INFINITY;
         }
-      float base[2];
+    }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < KPW / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+    }
+    // the same reference serves P, l and O, so the result does not depend on how old it is; P stays below 2^8
+    if (__any_sync(0xffffffffu, mx[0] - m[0] > 8.0f || mx[1] - m[1] > 8.0f)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-        base[i] = mx[i] == -INFINITY ? 0.f : mx[i];  // nothing seen yet: 2^(-inf - 0) = 0
-        const float alpha = exp2f(m[i] - base[i]);
-        m[i] = mx[i];
+        const float mn = fmaxf(m[i], mx[i]);
+        const float alpha = mn == -INFINITY ? 1.0f : attn::ex2_approx(m[i] - mn);
+        m[i] = mn;
         l[i] *= alpha;
 #pragma unroll
         for (int n = 0; n < DP / 8; ++n) {
@@ -236,79 +299,132 @@ paged_rows_kernel(const Params p) {
           o[n][2 * i + 1] *= alpha;
         }
       }
-      uint32_t pa[KPW / 16][4];
+    }
+    const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};  // nothing seen: 2^(-inf - 0) = 0
+    uint32_t pa[KPW / 16][4];
 #pragma unroll
-      for (int n = 0; n < KPW / 8; ++n) {
-        float e4[4];
+    for (int n = 0; n < KPW / 8; ++n) {
+      float e4[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          e4[e] = exp2f(s[n][e] - base[e >> 1]);
-          l[e >> 1] += e4[e];
-        }
-        const __half2 lo2 = __floats2half2_rn(e4[0], e4[1]), hi2 = __floats2half2_rn(e4[2], e4[3]);
-        pa[n >> 1][(n & 1) * 2] = *reinterpret_cast<const uint32_t *>(&lo2);
-        pa[n >> 1][(n & 1) * 2 + 1] = *reinterpret_cast<const uint32_t *>(&hi2);
+      for (int e = 0; e < 4; ++e) {
+        e4[e] = attn::ex2_approx(s[n][e] - base[e >> 1]);
+        l[e >> 1] += e4[e];
       }
+      pa[n >> 1][(n & 1) * 2] = attn::pack_f16x2(e4[0], e4[1]);
+      pa[n >> 1][(n & 1) * 2 + 1] = attn::pack_f16x2(e4[2], e4[3]);
+    }
+    const uint32_t vrow = (uint32_t)(kw * KPW + (lane & 7) + (((lane >> 3) & 1) << 3)), vx = vrow & 7;
+#pragma unroll
+    for (int n = 0; n < DP / 16; ++n) {
+      const uint32_t ch = (uint32_t)(n * 2) + (lane >> 4);
+      const uint32_t at = sv + (ch >> 3) * KV_CHUNK + vrow * 128 + (((ch & 7) ^ vx) << 4);
 #pragma unroll
       for (int k = 0; k < KPW / 16; ++k) {
-#pragma unroll
-        for (int n = 0; n < DP / 16; ++n) {
-          const int row = kw * KPW + k * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
-          const int c = n * 2 + (lane >> 4);
-          uint32_t b[4];
-          ldsm4t(sv + (uint32_t)(row * DP * 2 + ((c ^ (row & 7)) * 16)), b);
-          mma16816(o[2 * n], pa[k], b[0], b[1]);
-          mma16816(o[2 * n + 1], pa[k], b[2], b[3]);
-        }
+        uint32_t b[4];
+        ldsm4t(at + k * 16 * 128, b);
+        mma16816(o[2 * n], pa[k], b[0], b[1]);
+        mma16816(o[2 * n + 1], pa[k], b[2], b[3]);
       }
-      if (j + 3 < blocks) publish(j + 3, page_next);
     }
-    cp_async_wait<0>();
-    if (OWN && p.merge) pdl_wait();  // the prefix parts are complete
+  }
+
+  // The run is over: its part.  Runs of a tile are numbered by the CTAs that hold them.  All 128 consumer threads.
+  __device__ __forceinline__ void end(const Params &p, const Cursor &c, long long unit, long long per, float *xch) {
+    const long long tile_first = unit - c.j;
+    const int run = (int)((long long)blockIdx.x - tile_first / per);
+    const int part = (c.b < 0 ? 0 : p.prefix_parts) + run;
+    int *runs = c.b < 0 ? p.prefix_runs : p.own_runs;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      if (c.j == c.nb - 1 && runs && kw == 0 && (lane & 3) == 0 && row_ok[i]) runs[(int64_t)tok[i] * p.Hq + head[i]] = run + 1;
     }
-
     if (KW > 1) {
-      // join the key groups of a row group: maxima and sums first, then O group by group
-      __syncthreads();
-      float *sm = reinterpret_cast<float *>(smem);                 // [KW][ROWS] m, then l
-      float *so = sm + 2 * KW * ROWS;                              // [KW][ROWS][DP + 4]
+      // Join the key groups of a row group.  All scale to their common maximum; then key group w collects columns
+      // [w, w + 1) * DP / KW from the others, one of them a round (joining 16 columns of all groups at a time, between two
+      // barriers each, took 6.7 us a run; this takes a third).
+      constexpr int QC = DP / KW, PC = DP / 4;                 // columns a group keeps; of them a round
+      constexpr int PN = PC / 8, LD = PC + 2;                  // 8-column tiles, row pitch
+      float *sm = xch, *sl = xch + 64;                         // [KW][ROWS] each
+      float *so = xch + 128 + (kw * RW + rw) * 16 * LD;        // what this warp sends: its 16 rows
+      const int r0 = rw * 16 + (lane >> 2);
+      sync();
       if ((lane & 3) == 0) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int r = rw * 16 + (lane >> 2) + 8 * i;
-          sm[kw * ROWS + r] = m[i];
-          sm[(KW + kw) * ROWS + r] = l[i];
+          sm[kw * ROWS + r0 + 8 * i] = m[i];
+          sl[kw * ROWS + r0 + 8 * i] = l[i];
         }
       }
+      sync();
+      float mm[2], ll[2] = {0.f, 0.f};
 #pragma unroll
-      for (int n = 0; n < DP / 8; ++n)
+      for (int i = 0; i < 2; ++i) {
+        mm[i] = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = rw * 16 + (lane >> 2) + 8 * i;
-          *reinterpret_cast<float2 *>(so + (size_t)(kw * ROWS + r) * (DP + 4) + n * 8 + (lane & 3) * 2) =
-              make_float2(o[n][2 * i], o[n][2 * i + 1]);
-        }
-      __syncthreads();
-      for (int i = tid; i < ROWS * (DP / 4); i += THREADS) {
-        const int r = i / (DP / 4), d = (i % (DP / 4)) * 4;
-        if (row0 + r >= rows || d >= p.D) continue;
-        float mm = -INFINITY, ll = 0.f, f[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < KW; ++w) mm = fmaxf(mm, sm[w * ROWS + r]);
+        for (int w = 0; w < KW; ++w) mm[i] = fmaxf(mm[i], sm[w * ROWS + r0 + 8 * i]);
 #pragma unroll
         for (int w = 0; w < KW; ++w) {
-          const float lw = sm[(KW + w) * ROWS + r];
-          const float a = lw == 0.f ? 0.f : exp2f(sm[w * ROWS + r] - mm);
-          ll = fmaf(a, lw, ll);
-          const float4 v = *reinterpret_cast<const float4 *>(so + (size_t)(w * ROWS + r) * (DP + 4) + d);
-          f[0] = fmaf(a, v.x, f[0]); f[1] = fmaf(a, v.y, f[1]); f[2] = fmaf(a, v.z, f[2]); f[3] = fmaf(a, v.w, f[3]);
+          const float lw = sl[w * ROWS + r0 + 8 * i];
+          ll[i] += lw == 0.f ? 0.f : lw * attn::ex2_approx(sm[w * ROWS + r0 + 8 * i] - mm[i]);
         }
-        const int t = tok0 + (row0 + r) / p.G, hd = h * p.G + (row0 + r) % p.G;
-        store_row<4>(p, part, t, hd, d, f, mm, ll);
+        const float a = l[i] == 0.f ? 0.f : attn::ex2_approx(m[i] - mm[i]);
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n) {
+          o[n][2 * i] *= a;
+          o[n][2 * i + 1] *= a;
+        }
+      }
+      // fn(first 8-column tile of group w's columns) with a constant, so that O stays in registers
+      auto tile_of = [&](int w, auto &&fn) {
+        if (w == 0) fn(std::integral_constant<int, 0>{});
+        else if (w == 1) fn(std::integral_constant<int, (KW > 1 ? 1 : 0) * QC / 8>{});
+        else if (w == 2) fn(std::integral_constant<int, (KW > 2 ? 2 : 0) * QC / 8>{});
+        else fn(std::integral_constant<int, (KW > 3 ? 3 : 0) * QC / 8>{});
+      };
+#pragma unroll
+      for (int pc = 0; pc < QC / PC; ++pc) {
+        float f[PN][4];
+        tile_of(kw, [&](auto t) {
+#pragma unroll
+          for (int n = 0; n < PN; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[n][e] = o[decltype(t)::value + pc * PN + n][e];
+        });
+#pragma unroll 1
+        for (int d = 1; d < KW; ++d) {
+          // to group (kw + d) % KW its columns; from group (kw - d) % KW this warp's
+          tile_of((kw + d) % KW, [&](auto t) {
+#pragma unroll
+            for (int n = 0; n < PN; ++n)
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<float2 *>(so + ((lane >> 2) + 8 * i) * LD + n * 8 + (lane & 3) * 2) =
+                    make_float2(o[decltype(t)::value + pc * PN + n][2 * i], o[decltype(t)::value + pc * PN + n][2 * i + 1]);
+          });
+          sync();
+          const float *in = xch + 128 + (((kw + KW - d) % KW) * RW + rw) * 16 * LD;
+#pragma unroll
+          for (int n = 0; n < PN; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 v = *reinterpret_cast<const float2 *>(in + ((lane >> 2) + 8 * i) * LD + n * 8 + (lane & 3) * 2);
+              f[n][2 * i] += v.x;
+              f[n][2 * i + 1] += v.y;
+            }
+          sync();
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!row_ok[i]) continue;
+#pragma unroll
+          for (int n = 0; n < PN; ++n) {
+            const int d = kw * QC + pc * PC + n * 8 + (lane & 3) * 2;
+            float v[2] = {f[n][2 * i], f[n][2 * i + 1]};
+            if (d < p.D) store_row<2>(p, part, tok[i], head[i], d, v, mm[i], ll[i]);
+          }
+        }
       }
     } else {
 #pragma unroll
@@ -323,39 +439,282 @@ paged_rows_kernel(const Params p) {
       }
     }
   }
-  if (OWN) {
-    pdl_wait();  // whoever waits for this launch waits for the prefix launch too
-    pdl_launch_dependents();
+  // Barrier of the consumer warps.  They leave their loop together in every case (a wait that gave up does not end it).
+  static __device__ __forceinline__ void sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+};
+
+// ---- blocks fetched by TMA: warps 0-3 consume, warp 4 produces
+template <int DP, int RW>
+__global__ void __launch_bounds__(160, RowCfg<DP>::PER_SM)
+paged_stream_tma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Params p) {
+  using cfg = RowCfg<DP>;
+  constexpr int BN = cfg::BN, ST = cfg::STAGES;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw = tc::smem_u32(smem_raw), s0 = (raw + 1023u) & ~1023u;
+  uint8_t *smem = smem_raw + (s0 - raw);
+  auto full = [&](int i) { return s0 + cfg::BARS + 8 * i; };
+  auto empty = [&](int i) { return s0 + cfg::BARS + 8 * (ST + i); };
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + cfg::BARS + 2 * ST * 8);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      tc::mbar_init(full(i), 1);
+      tc::mbar_init(empty(i), 4);
+    }
+    *abort_flag = 0;
+    tc::fence_barrier_init();
+    tc::prefetch_tensormap(&tmK);
+    tc::prefetch_tensormap(&tmV);
   }
+  // After the call's own tensor-core launch this one need not wait: it does not touch what that one writes, and that
+  // one lets it start only when all that came before is complete.
+  if (!p.follows_prefix) pdl_wait();
+  long long start, stop, per;
+  Cursor c;
+  find_stretch<RW, 160>(p, start, stop, per, c);   // its barriers also publish the ones set up above
+  if (start < stop) {
+    const int units = (int)(stop - start);
+    if (warp == 4) {
+      const int pieces = BN / p.piece;
+      auto lookup = [&](int u, int &slot) {
+        int page = p.num_pages;                     // no key there: reads as zeros
+        slot = 0;
+        if (lane < pieces && u < units) {
+          const int key = c.j * BN + lane * p.piece;
+          if (key < end_of<RW>(p, c)) {
+            const int pi = key / p.page_size;
+            slot = key - pi * p.page_size;
+            const int got = c.b < 0 ? p.prefix_pages[pi] : p.table[(int64_t)c.b * p.table_stride + pi];
+            if ((unsigned)got < (unsigned)p.num_pages) page = got;
+            else atomicExch(&g_paged_status, (int)HEXB_ERR_BAD_ARG);
+          }
+        }
+        return page;
+      };
+      int slot_next, page_next = lookup(0, slot_next);
+      for (int u = 0; u < units; ++u) {
+        const int st = u % ST, page = page_next, slot = slot_next, h = c.h;
+        if (u + 1 < units) advance<RW>(p, c);
+        page_next = lookup(u + 1, slot_next);
+        if (!tc::mbar_wait(empty(st), (uint32_t)(u / ST + 1) & 1u, abort_flag)) break;
+        if (lane == 0) tc::mbar_arrive_expect_tx(full(st), 2 * cfg::KV);
+        __syncwarp();
+        if (lane < pieces) {
+          const uint32_t dst = s0 + (uint32_t)st * 2 * cfg::KV + (uint32_t)(lane * p.piece) * 128u;
+#pragma unroll
+          for (int k = 0; k < DP / 64; ++k) {
+            tc::tma_load_4d(dst + k * cfg::KV_CHUNK, &tmK, k * 64, h, slot, page, full(st));
+            tc::tma_load_4d(dst + cfg::KV + k * cfg::KV_CHUNK, &tmV, k * 64, h, slot, page, full(st));
+          }
+        }
+      }
+    } else {
+      Run<DP, RW> r;
+      r.lane = lane;
+      r.rw = warp % RW;
+      r.kw = warp / RW;
+      float *xch = reinterpret_cast<float *>(smem + cfg::XCH);
+      int end = 0;
+      for (int u = 0; u < units; ++u) {
+        if (u == 0 || c.j == 0) {
+          r.begin(p, c);
+          end = end_of<RW>(p, c);
+        }
+        const int st = u % ST;
+        const uint32_t sk = s0 + (uint32_t)st * 2 * cfg::KV, sv = sk + cfg::KV;
+        // Should it give up, the loop goes on, without waiting further, over whatever the stage holds: the warps meet at
+        // barriers, and the status word tells the host.
+        tc::mbar_wait(full(st), (uint32_t)(u / ST) & 1u, abort_flag);
+        // this warp's keys behind the last one: whatever the slots hold -- NaN, perhaps -- must not meet a weight of 0
+        const int k0 = r.kw * Run<DP, RW>::KPW, k1 = k0 + Run<DP, RW>::KPW;
+        const int filled = max(end - c.j * BN, 0);
+        if (filled < k1) {
+          const int from = max(filled, k0);
+          __syncwarp();
+          for (int i = lane; i < (k1 - from) * (DP / 8); i += 32) {
+            const int row = from + i / (DP / 8), ch = i % (DP / 8);
+            *reinterpret_cast<uint4 *>(smem + (sv - s0) + (ch >> 3) * cfg::KV_CHUNK + row * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          __syncwarp();   // (warps that share the keys write the same zeros)
+        }
+        r.step(p, c, end, sk, sv);
+        if (filled < k1) tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(empty(st));
+        if (c.j == c.nb - 1 || u == units - 1) r.end(p, c, start + u, per, xch);
+        if (u + 1 < units) advance<RW>(p, c);
+      }
+    }
+    if (*abort_flag) {
+      for (int i = 0; i < 200; ++i) __nanosleep(1000);  // lets copies in flight land before the CTA's memory goes
+      if (threadIdx.x == 0) atomicExch(&g_paged_status, (int)HEXB_ERR_TIMEOUT);
+    }
+  }
+  pdl_wait();  // whoever waits for this launch waits for the tensor-core launch too
+  pdl_launch_dependents();
+}
+
+// ---- blocks copied by cp.async
+template <int DP, int RW>
+__global__ void __launch_bounds__(THREADS, RowCfg<DP>::PER_SM)
+paged_stream_kernel(const Params p) {
+  using cfg = RowCfg<DP>;
+  constexpr int BN = cfg::BN;
+  constexpr int CH = DP / 8;  // 16-byte chunks of a row
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t s0 = (uint32_t)__cvta_generic_to_shared(smem);
+  int64_t *offs = reinterpret_cast<int64_t *>(smem + cfg::OFFS);
+  const int tid = threadIdx.x, warp = tid >> 5;
+  if (!p.follows_prefix) pdl_wait();
+  long long start, stop, per;
+  Cursor cc, cl;                        // the unit being computed, the one whose pages are looked up
+  find_stretch<RW, THREADS>(p, start, stop, per, cc);
+  if (start < stop) {
+    const int units = (int)(stop - start);
+    int looked = 0, fetched = 0;
+    cl = cc;
+    auto lookup = [&]() -> int {        // thread tid < 64: page of key tid of unit `looked`
+      int page = -1;
+      if (looked < units && tid < BN) {
+        const int key = cl.j * BN + tid;
+        if (key < end_of<RW>(p, cl)) {
+          const int pi = key / p.page_size;
+          page = cl.b < 0 ? p.prefix_pages[pi] : p.table[(int64_t)cl.b * p.table_stride + pi];
+        }
+      }
+      return page;
+    };
+    auto publish = [&](int page) {      // row offsets of unit `looked`; then the next one's turn
+      if (looked < units) {
+        if (tid < BN) {
+          const int key = cl.j * BN + tid;
+          int64_t ko = -1, vo = -1;
+          if (key < end_of<RW>(p, cl)) {
+            if ((unsigned)page < (unsigned)p.num_pages) {
+              const int64_t in = key % p.page_size;
+              ko = (int64_t)page * p.sk_p + in * p.sk_s + (int64_t)cl.h * p.sk_h;
+              vo = (int64_t)page * p.sv_p + in * p.sv_s + (int64_t)cl.h * p.sv_h;
+            } else {
+              atomicExch(&g_paged_status, (int)HEXB_ERR_BAD_ARG);
+            }
+          }
+          int64_t *o = offs + (looked & 1) * 2 * BN;
+          o[tid] = ko;
+          o[BN + tid] = vo;
+        }
+        advance<RW>(p, cl);
+      }
+      ++looked;
+    };
+    auto fetch = [&]() {
+      if (fetched < units) {
+        const int64_t *o = offs + (fetched & 1) * 2 * BN;
+        const int c = tid % CH;
+        const uint32_t st = s0 + (uint32_t)(fetched % cfg::STAGES) * 2 * cfg::KV + (c >> 3) * cfg::KV_CHUNK;
+        const bool col = c * 8 < p.D;
+#pragma unroll
+        for (int i = 0; i < BN * CH / THREADS; ++i) {
+          const int row = tid / CH + i * (THREADS / CH);
+          const uint32_t dst = st + (uint32_t)(row * 128 + (((c & 7) ^ (row & 7)) * 16));
+          const int64_t ko = o[row], vo = o[BN + row];
+          const bool kv = col && ko >= 0;
+          cp_async16(dst, p.k + (kv ? ko + c * 8 : 0), kv);
+          cp_async16(dst + cfg::KV, p.v + (kv ? vo + c * 8 : 0), kv);
+        }
+      }
+      ++fetched;
+      cp_async_commit();
+    };
+    int page_next;
+    publish(lookup());
+    publish(lookup());
+    __syncthreads();
+    fetch();
+    fetch();
+    page_next = lookup();
+    __syncthreads();
+    publish(page_next);
+
+    Run<DP, RW> r;
+    r.lane = tid & 31;
+    r.rw = warp % RW;
+    r.kw = warp / RW;
+    int end = 0;
+    for (int u = 0; u < units; ++u) {
+      if (u == 0 || cc.j == 0) {
+        r.begin(p, cc);
+        end = end_of<RW>(p, cc);
+      }
+      cp_async_wait<1>();
+      __syncthreads();  // unit u landed for all; unit u - 1's readers are done; offsets of u + 2 are visible
+      fetch();
+      page_next = lookup();
+      const uint32_t sk = s0 + (uint32_t)(u % cfg::STAGES) * 2 * cfg::KV;
+      r.step(p, cc, end, sk, sk + cfg::KV);
+      publish(page_next);
+      if (cc.j == cc.nb - 1 || u == units - 1) r.end(p, cc, start + u, per, reinterpret_cast<float *>(smem + cfg::XCH));
+      if (u + 1 < units) advance<RW>(p, cc);
+    }
+    cp_async_wait<0>();
+  }
+  pdl_wait();  // whoever waits for this launch waits for the tensor-core launch too
+  pdl_launch_dependents();
 }
 
 // ------------------------------------------------------------------ join of the parts
-// One warp per (token, query head).
+// One warp per (token, query head); LPR lanes hold the row, the 32 / LPR groups of lanes take every so many-th part.
+template <int LPR>
 __global__ void __launch_bounds__(128) paged_join_kernel(const Params p) {
   pdl_wait();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, sub = lane / LPR, col = lane % LPR;
+  constexpr int SUBS = 32 / LPR;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int t = (int)(row / p.Hq), hd = (int)(row - (int64_t)t * p.Hq);
   if (t >= tokens_used(p)) return;
-  const int parts = p.prefix_parts + p.own_parts;
   const int64_t n = (int64_t)p.T * p.Hq;
+  // the parts of a row: those of the prefix, then those of its own keys; each side may hold fewer runs than slots
+  const int np = p.prefix_runs ? min(max(p.prefix_runs[row], 0), p.prefix_parts) : p.prefix_parts;
+  const int no = p.own_runs ? min(max(p.own_runs[row], 0), p.own_parts) : p.own_parts;
+  const int parts = np + no;
+  auto slot = [&](int i) { return i < np ? i : p.prefix_parts + i - np; };
   float mm = -INFINITY;
-  for (int i = lane; i < parts; i += 32) mm = fmaxf(mm, p.part_ml[i * n + row].x);
+  for (int i = lane; i < parts; i += 32) {
+    const float2 ml = p.part_ml[slot(i) * n + row];
+    if (ml.y != 0.f) mm = fmaxf(mm, ml.x);
+  }
   mm = warp_max(mm);
-  for (int d = lane * 4; d < p.D; d += 128) {
+  for (int d0 = 0; d0 < p.D; d0 += LPR * 4) {
+    const int d = d0 + col * 4;
     float f[4] = {0.f, 0.f, 0.f, 0.f}, ll = 0.f;
-    for (int i = 0; i < parts; ++i) {
-      const float2 ml = p.part_ml[i * n + row];
-      if (ml.y == 0.f) continue;  // no key seen: no O either
-      const float a = exp2f(ml.x - mm);
-      ll = fmaf(a, ml.y, ll);
-      const float4 v = *reinterpret_cast<const float4 *>(p.part_o + (i * n + row) * p.D + d);
-      f[0] = fmaf(a, v.x, f[0]); f[1] = fmaf(a, v.y, f[1]); f[2] = fmaf(a, v.z, f[2]); f[3] = fmaf(a, v.w, f[3]);
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      float2 ml = make_float2(0.f, 0.f);
+      if (i0 + lane < parts) ml = p.part_ml[slot(i0 + lane) * n + row];
+      const float w = ml.y == 0.f ? 0.f : exp2f(ml.x - mm);  // no key seen: no O either
+      ll += warp_sum(w * ml.y);
+      const int m = min(32, parts - i0);
+#pragma unroll 8
+      for (int i = 0; i < m; i += SUBS) {
+        // every lane loads, from a slot in bounds, and then selects: loads behind a branch would not overlap
+        const int k = i + sub;
+        const float a = __shfl_sync(0xffffffffu, w, k & 31);
+        const float4 v = __ldcs(reinterpret_cast<const float4 *>(p.part_o + (slot(i0 + min(k, m - 1)) * n + row) * p.D + min(d, p.D - 4)));
+        const bool use = k < m && a != 0.f;
+        f[0] = fmaf(use ? a : 0.f, use ? v.x : 0.f, f[0]);
+        f[1] = fmaf(use ? a : 0.f, use ? v.y : 0.f, f[1]);
+        f[2] = fmaf(use ? a : 0.f, use ? v.z : 0.f, f[2]);
+        f[3] = fmaf(use ? a : 0.f, use ? v.w : 0.f, f[3]);
+      }
     }
+#pragma unroll
+    for (int s = LPR; s < 32; s <<= 1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] += __shfl_xor_sync(0xffffffffu, f[e], s);
     const float inv = ll == 0.f ? 0.f : 1.0f / ll;
-    __half2 *o = reinterpret_cast<__half2 *>(p.out + (int64_t)t * p.so_t + (int64_t)hd * p.so_h + d);
-    o[0] = __floats2half2_rn(f[0] * inv, f[1] * inv);
-    o[1] = __floats2half2_rn(f[2] * inv, f[3] * inv);
+    if (sub == 0 && d < p.D) {
+      __half2 *o = reinterpret_cast<__half2 *>(p.out + (int64_t)t * p.so_t + (int64_t)hd * p.so_h + d);
+      o[0] = __floats2half2_rn(f[0] * inv, f[1] * inv);
+      o[1] = __floats2half2_rn(f[2] * inv, f[3] * inv);
+    }
   }
 }
 
@@ -365,102 +724,107 @@ static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // How a call is cut.  A function of the sizes alone, so that the workspace query and the launch agree.
 struct Plan {
   bool seq, tc_prefix;            // tensor-core forms
-  int prefix_parts, prefix_chunk, own_parts;
-  int prefix_rw, own_rw;
+  bool stream;                    // the stream of key blocks: own keys, and the prefix unless tc_prefix
+  bool stream_prefix;
+  int prefix_parts, own_parts;    // slots
+  int rw;
+  int64_t ctas;                   // of the stream
+  bool tma;                       // the stream's blocks by TMA
   int tile_tokens, piece;
   int parts() const { return prefix_parts + own_parts; }
-  bool merge() const { return prefix_parts > 0 && own_parts == 1; }
 };
 
 static int rw_for(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+static int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
 static Plan make_plan(const hexb_paged_attention_desc *d, int sm_count) {
   Plan pl = {};
   const int64_t G = d->Hq / d->Hkv, capacity = d->table_width * d->page_size;
   const int64_t mq = d->max_q > 0 ? d->max_q : ceil_div(d->T, d->B);
-  const int64_t pblocks = ceil_div(d->prefix_len, 64);
-  // The tensor-core forms: what TMA can address (page pieces of at least the 8 rows of a swizzle atom, no stride of 0), a
-  // positive scale, and enough rows to fill half of a 128-row tile; below that the key stream, not the products, is
+  const int64_t pblocks = ceil_div(d->prefix_len, 64), oblocks = ceil_div(capacity, 64);
+  // What TMA can address: page pieces of at least the 8 rows of a swizzle atom, no stride of 0.
+  // The tensor-core forms want besides: a positive scale, and enough rows to fill half of a 128-row tile; below that the key stream, not the products, is
   // what takes the time, and the small tiles of mma.sync read it as fast.
   pl.piece = (int)(d->page_size & -d->page_size);
   if (pl.piece > 64) pl.piece = 64;
-  bool tc_ok = (d->D == 64 || d->D == 128) && pl.piece >= 8 && d->sm_scale > 0.f && G <= 128;
-  const int64_t dims[10] = {d->T, d->Hq, d->num_pages, d->page_size, d->Hkv, d->num_pages, d->page_size, d->Hkv, 1, 1};
-  for (int i = 0; i < 8; ++i) tc_ok = tc_ok && (dims[i] <= 1 || (d->strides[i] > 0 && d->strides[i] < ((int64_t)1 << 38)));
-  tc_ok = tc_ok && (d->Hkv <= 1 || d->strides[1] * G < ((int64_t)1 << 38));
+  bool tma_ok = (d->D == 64 || d->D == 128) && pl.piece >= 8;
+  const int64_t dims[8] = {d->T, d->Hq, d->num_pages, d->page_size, d->Hkv, d->num_pages, d->page_size, d->Hkv};
+  auto fits = [&](int i) { return dims[i] <= 1 || (d->strides[i] > 0 && d->strides[i] < ((int64_t)1 << 38)); };
+  for (int i = 2; i < 8; ++i) tma_ok = tma_ok && fits(i);
+  pl.tma = tma_ok;
+  const bool tc_ok = tma_ok && fits(0) && fits(1) && d->sm_scale > 0.f && G <= 128 && (d->Hkv <= 1 || d->strides[1] * G < ((int64_t)1 << 38));
   pl.tile_tokens = tc_ok ? (int)(128 / G) : 0;
   if (tc_ok && mq * G >= 64 && capacity > 0) {
     // tiles of one sequence each, over prefix and own keys: cut the axis only when the tiles leave SMs idle
     pl.seq = true;
     const int64_t tiles = d->B * ceil_div(mq, pl.tile_tokens) * d->Hkv;
-    int64_t parts = 2 * sm_count / tiles;
-    const int64_t most = (pblocks + capacity / 64) / 8;
-    if (parts > most) parts = most;
-    if (parts > 32) parts = 32;
-    pl.prefix_parts = parts > 1 ? (int)parts : 1;
+    pl.prefix_parts = (int)clamp64(2 * sm_count / tiles, 1, clamp64((pblocks + oblocks) / 8, 1, 32));
     return pl;
   }
+  const int per_sm = d->D <= 64 ? 4 : d->D <= 128 ? 2 : 1;
   if (d->prefix_len > 0 && tc_ok && d->T * G >= 64) {
-    // One CTA an SM when own keys follow: their launch shares the SMs and streams beside the products.
     pl.tc_prefix = true;
     const int64_t tiles = (int64_t)ceil_div(d->T, pl.tile_tokens) * d->Hkv;
-    int64_t parts = (capacity > 0 ? 1 : 2) * sm_count / tiles;
-    if (parts < 1) parts = 1;
-    if (parts > 64) parts = 64;
-    if (parts > (pblocks + 1) / 2) parts = (pblocks + 1) / 2;
-    const int64_t per = ceil_div(pblocks, parts);
-    pl.prefix_parts = ceil_div(pblocks, per);
-  } else if (d->prefix_len > 0) {
-    const int per_sm = d->D <= 64 ? 4 : d->D <= 128 ? 2 : 1;
-    const int64_t want = (int64_t)sm_count * per_sm * 2;
-    pl.prefix_rw = rw_for(d->T * G);
-    const int64_t tiles = (int64_t)ceil_div(d->T * G, 16 * pl.prefix_rw) * d->Hkv;
-    int64_t parts = ceil_div(want, tiles);
-    const int64_t most = ceil_div(d->prefix_len, 256);
-    if (parts > most) parts = most;
-    if (parts > 64) parts = 64;
-    pl.prefix_chunk = ceil_div(ceil_div(d->prefix_len, parts), 64) * 64;
-    pl.prefix_parts = ceil_div(d->prefix_len, pl.prefix_chunk);
+    const int64_t parts = clamp64(2 * sm_count / tiles, 1, clamp64((pblocks + 1) / 2, 1, 64));
+    pl.prefix_parts = ceil_div(pblocks, ceil_div(pblocks, parts));
   }
-  if (capacity > 0) {
-    pl.own_rw = rw_for(mq * G);
-    const int64_t tiles = (int64_t)d->B * ceil_div(mq * G, 16 * pl.own_rw) * d->Hkv;
-    int64_t parts = sm_count * 2 / tiles;   // one part (and no join launch) once the tiles fill the SMs
-    const int64_t most = ceil_div(capacity, 256);
-    if (parts > most) parts = most;
-    if (parts > 64) parts = 64;
-    pl.own_parts = parts > 1 ? (int)parts : 1;
+  pl.stream_prefix = d->prefix_len > 0 && !pl.tc_prefix;
+  pl.stream = pl.stream_prefix || capacity > 0;
+  if (pl.stream) {
+    pl.rw = rw_for(mq * G);
+    if ((pl.stream_prefix && d->T * G > 128) || d->D > 128) pl.rw = 4;
+    const int64_t rows = 16 * pl.rw;
+    const int64_t fit = (int64_t)sm_count * per_sm;
+    // units at most (a tile of every sequence may be cut short), so that a small call launches no idle CTA
+    const int64_t ptiles = pl.stream_prefix ? ceil_div(d->T * G, rows) * d->Hkv : 0;
+    const int64_t otiles = (ceil_div(d->T * G, rows) + d->B) * d->Hkv;
+    const double most = (double)ptiles * pblocks + (double)otiles * (oblocks > 1 ? oblocks : 1);
+    pl.ctas = most < (double)fit ? (int64_t)most : fit;
+    if (pl.ctas < 1) pl.ctas = 1;
+    // Slots for the runs of a tile: twice its share of the CTAs (ragged lengths); if some tile is longer still, the
+    // kernel gives every CTA so many units that its runs fit.
+    const int64_t tiles = ptiles + (capacity > 0 ? d->B * ceil_div(mq * G, rows) * d->Hkv : 0);
+    const int64_t slots = clamp64(2 + 2 * pl.ctas / tiles, 3, 64);
+    if (pl.stream_prefix) pl.prefix_parts = (int)clamp64(pblocks, 1, slots);
+    if (capacity > 0) pl.own_parts = (int)clamp64(oblocks, 1, slots);
   }
   return pl;
 }
 
 static size_t ws_need(const hexb_paged_attention_desc *d, const Plan &pl) {
   if (pl.parts() < 2) return 0;
-  const size_t parts = pl.merge() ? (size_t)pl.prefix_parts : (size_t)pl.parts();
-  return parts * (size_t)d->T * d->Hq * ((size_t)d->D * 4 + 8) + 256;
+  return (size_t)pl.parts() * d->T * d->Hq * ((size_t)d->D * 4 + 8) + (size_t)d->T * d->Hq * 8 + 256;
 }
 
-template <int DP, int RW, bool OWN>
-static int launch_rows(const Params &p, dim3 grid, cudaStream_t st) {
+template <int DP, int RW>
+static int launch_stream(const Params &p, const CUtensorMap *tm, dim3 grid, cudaStream_t st) {
   static PerDeviceOnce once;
   int dev = 0;
   HEXB_CUDA_OK(cudaGetDevice(&dev));
+  using cfg = RowCfg<DP>;
   if (!once.is_done(dev)) {
-    HEXB_CUDA_OK(cudaFuncSetAttribute(paged_rows_kernel<DP, RW, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowCfg<DP>::SMEM));
+    HEXB_CUDA_OK(cudaFuncSetAttribute(paged_stream_kernel<DP, RW>, cudaFuncAttributeMaxDynamicSharedMemorySize, cfg::SMEM));
+    if constexpr (DP <= 128)
+      HEXB_CUDA_OK(cudaFuncSetAttribute(paged_stream_tma_kernel<DP, RW>, cudaFuncAttributeMaxDynamicSharedMemorySize, cfg::SMEM_TMA));
     once.mark(dev);
   }
-  HEXB_CUDA_OK(launch_pdl(paged_rows_kernel<DP, RW, OWN>, grid, dim3(THREADS), (size_t)RowCfg<DP>::SMEM, st, p));
-  return check_launch("paged_rows");
+  if constexpr (DP <= 128) {
+    if (tm) {
+      HEXB_CUDA_OK(launch_pdl(paged_stream_tma_kernel<DP, RW>, grid, dim3(160), (size_t)cfg::SMEM_TMA, st, tm[0], tm[1], p));
+      return check_launch("paged_stream_tma");
+    }
+  }
+  HEXB_CUDA_OK(launch_pdl(paged_stream_kernel<DP, RW>, grid, dim3(THREADS), (size_t)cfg::SMEM, st, p));
+  return check_launch("paged_stream");
 }
 
-template <bool OWN>
-static int dispatch_rows(const Params &p, int rw, dim3 grid, cudaStream_t st) {
-#define HEXB_ROWS(DP)                                                   \
-  return rw == 1 ? launch_rows<DP, 1, OWN>(p, grid, st)                 \
-                 : rw == 2 ? launch_rows<DP, 2, OWN>(p, grid, st) : launch_rows<DP, 4, OWN>(p, grid, st)
+static int dispatch_stream(const Params &p, int rw, const CUtensorMap *tm, dim3 grid, cudaStream_t st) {
+#define HEXB_ROWS(DP)                                                  \
+  return rw == 1 ? launch_stream<DP, 1>(p, tm, grid, st)               \
+                 : rw == 2 ? launch_stream<DP, 2>(p, tm, grid, st) : launch_stream<DP, 4>(p, tm, grid, st)
   if (p.D <= 64) HEXB_ROWS(64);
   if (p.D <= 128) HEXB_ROWS(128);
-  HEXB_ROWS(256);
+  return launch_stream<256, 4>(p, tm, grid, st);
 #undef HEXB_ROWS
 }
 
@@ -525,46 +889,40 @@ extern "C" int hexb_paged_attention_f16(const hexb_paged_attention_desc *d, void
   p.T = (int)d->T; p.B = (int)d->B; p.Hq = (int)d->Hq; p.G = (int)(d->Hq / d->Hkv); p.D = (int)d->D;
   p.prefix_len = (int)d->prefix_len; p.page_size = (int)d->page_size; p.num_pages = (int)d->num_pages;
   p.own_capacity = (int)(d->table_width * d->page_size);
-  p.prefix_parts = pl.prefix_parts; p.prefix_chunk = pl.prefix_chunk; p.own_parts = pl.own_parts;
+  p.prefix_parts = pl.prefix_parts; p.own_parts = pl.own_parts;
+  p.nseq = p.own_capacity ? p.B : 0;
   p.scale_log2 = d->sm_scale * 1.44269504f;
   p.tile_tokens = pl.tile_tokens;
   p.piece = pl.piece;
   if (need) {
-    const size_t n = (size_t)(pl.merge() ? pl.prefix_parts : pl.parts()) * d->T * d->Hq;
+    const size_t rows = (size_t)d->T * d->Hq, n = (size_t)pl.parts() * rows;
     uint8_t *w = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~(uintptr_t)15);
     p.part_o = reinterpret_cast<float *>(w);
     p.part_ml = reinterpret_cast<float2 *>(w + n * d->D * 4);
+    int *runs = reinterpret_cast<int *>(w + n * (d->D * 4 + 8));
+    if (pl.stream_prefix) p.prefix_runs = runs;
+    if (pl.own_parts) p.own_runs = runs + rows;
   }
   cudaStream_t st = (cudaStream_t)stream;
   const int64_t mq = d->max_q > 0 ? d->max_q : paged::ceil_div(d->T, d->B);
-  auto grid_of = [&](int64_t x, int64_t y, dim3 *g) {
-    if (x > 0x7fffffff || y > 65535) return false;
-    *g = dim3((unsigned)x, (unsigned)y, (unsigned)d->Hkv);
-    return true;
-  };
-  dim3 grid;
-  if (pl.seq) {
-    if (!grid_of(paged::ceil_div(mq, pl.tile_tokens), (int64_t)pl.prefix_parts * d->B, &grid)) return HEXB_ERR_UNSUPPORTED;
-    if (int e = paged::tc_launch(p, (int)d->Hkv, true, grid, st)) return e;
-  } else if (pl.tc_prefix) {
-    if (!grid_of(paged::ceil_div(d->T, pl.tile_tokens), pl.prefix_parts, &grid)) return HEXB_ERR_UNSUPPORTED;
-    if (int e = paged::tc_launch(p, (int)d->Hkv, false, grid, st)) return e;
-  } else if (pl.prefix_parts) {
-    if (!grid_of(paged::ceil_div(d->T * p.G, 16 * pl.prefix_rw), pl.prefix_parts, &grid)) return HEXB_ERR_UNSUPPORTED;
-    if (int e = paged::dispatch_rows<false>(p, pl.prefix_rw, grid, st)) return e;
+  if (pl.seq || pl.tc_prefix) {
+    const int64_t x = paged::ceil_div(pl.seq ? mq : d->T, pl.tile_tokens), y = (int64_t)pl.prefix_parts * (pl.seq ? d->B : 1);
+    if (y > 65535) return HEXB_ERR_UNSUPPORTED;
+    if (int e = paged::tc_launch(p, (int)d->Hkv, pl.seq, dim3((unsigned)x, (unsigned)y, (unsigned)d->Hkv), st)) return e;
   }
-  if (pl.own_parts) {
-    if (!grid_of(paged::ceil_div(mq * p.G, 16 * pl.own_rw), (int64_t)pl.own_parts * d->B, &grid)) return HEXB_ERR_UNSUPPORTED;
-    paged::Params po = p;
-    po.follows_prefix = pl.prefix_parts > 0;
-    po.merge = pl.merge();
-    if (int e = paged::dispatch_rows<true>(po, pl.own_rw, grid, st)) return e;
-    if (pl.merge()) return HEXB_OK;
+  if (pl.stream) {
+    p.follows_prefix = pl.tc_prefix;
+    p.stream_prefix = pl.stream_prefix;
+    CUtensorMap tm[2];
+    if (pl.tma)
+      if (int e = paged::cache_maps(p, (int)d->Hkv, tm)) return e;
+    if (int e = paged::dispatch_stream(p, pl.rw, pl.tma ? tm : nullptr, dim3((unsigned)pl.ctas), st)) return e;
   }
   if (pl.parts() != 1) {
     // also the call without any key: its rows are set to zero
-    const int64_t rows = d->T * d->Hq;
-    HEXB_CUDA_OK(launch_pdl(paged::paged_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p));
+    const dim3 grid((unsigned)((d->T * d->Hq + 3) / 4));
+    if (d->D <= 64) HEXB_CUDA_OK(launch_pdl(paged::paged_join_kernel<16>, grid, dim3(128), 0, st, p));
+    else HEXB_CUDA_OK(launch_pdl(paged::paged_join_kernel<32>, grid, dim3(128), 0, st, p));
     return check_launch("paged_join");
   }
   return HEXB_OK;

@@ -1,6 +1,6 @@
 // Parameters and device helpers shared by the paged-attention kernels.
 #pragma once
-#include "common.cuh"
+#include "tc_sm100.cuh"
 
 namespace hexb {
 
@@ -19,13 +19,15 @@ struct Params {
   int64_t table_stride;
   int T, B, Hq, G, D;
   int prefix_len, page_size, num_pages, own_capacity;
-  int prefix_parts, prefix_chunk, own_parts;
+  int prefix_parts, own_parts;        // slots for parts
   float scale_log2;
   float *part_o;                      // [part][T * Hq][D]
   float2 *part_ml;                    // [part][T * Hq]: row maximum (base 2) and sum
   int tile_tokens, piece;             // tensor-core form: tokens of a tile, keys of one TMA box
-  int follows_prefix;                 // this launch may start while the call's prefix launch is still running
-  int merge;                          // and joins its parts with its own result instead of storing a part
+  int follows_prefix;                 // the stream follows the call's tensor-core launch over the prefix
+  int nseq;                           // sequences in the stream: B, or 0 without own keys
+  int stream_prefix;                  // the stream of key blocks covers the prefix too
+  int *prefix_runs, *own_runs;        // [T * Hq]: parts in use, or NULL: all slots are
 };
 
 // Tokens [tok0, tok0 + n) of sequence b.  Offsets are data on the device: whatever they hold, the rows
@@ -49,50 +51,11 @@ __device__ __forceinline__ int seq_len(const Params &p, int b) {
   return min(max(n, 0), p.own_capacity);
 }
 
-// out = join of the prefix parts and (f, m, l), elements d .. d + W - 1 of one row.
-template <int W>
-__device__ __forceinline__ void merge_row(const Params &p, int t, int hd, int d, float (&f)[W], float m, float l) {
-  const int64_t n = (int64_t)p.T * p.Hq, row = (int64_t)t * p.Hq + hd;
-  float mm = l == 0.f ? -INFINITY : m;
-  for (int i = 0; i < p.prefix_parts; ++i) {
-    const float2 ml = __ldcg(&p.part_ml[i * n + row]);
-    if (ml.y != 0.f) mm = fmaxf(mm, ml.x);
-  }
-  const float a = l == 0.f ? 0.f : exp2f(m - mm);
-  float ll = l * a;
-#pragma unroll
-  for (int e = 0; e < W; ++e) f[e] = l == 0.f ? 0.f : f[e] * a;
-#pragma unroll 4
-  for (int i = 0; i < p.prefix_parts; ++i) {
-    const float2 ml = __ldcg(&p.part_ml[i * n + row]);
-    if (ml.y == 0.f) continue;
-    const float w = exp2f(ml.x - mm);
-    ll = fmaf(w, ml.y, ll);
-    const float *o = p.part_o + (i * n + row) * p.D + d;
-    float v[W];
-    if (W == 4) {
-      const float4 q = __ldcg(reinterpret_cast<const float4 *>(o));
-      v[0] = q.x; v[1] = q.y; v[W - 2] = q.z; v[W - 1] = q.w;
-    } else {
-      const float2 q = __ldcg(reinterpret_cast<const float2 *>(o));
-      v[0] = q.x; v[1] = q.y;
-    }
-#pragma unroll
-    for (int e = 0; e < W; ++e) f[e] = fmaf(w, v[e], f[e]);
-  }
-  const float inv = ll == 0.f ? 0.f : 1.0f / ll;
-  __half2 *o = reinterpret_cast<__half2 *>(p.out + (int64_t)t * p.so_t + (int64_t)hd * p.so_h + d);
-#pragma unroll
-  for (int e = 0; e < W; e += 2) o[e / 2] = __floats2half2_rn(f[e] * inv, f[e + 1] * inv);
-}
-
 // Result of a part, elements d .. d + W - 1 of one row, or the output itself when the call has one part.  l == 0 marks a
 // part in which the row saw no key: its O is neither stored nor read.
 template <int W>
 __device__ __forceinline__ void store_row(const Params &p, int part, int t, int hd, int d, float (&f)[W], float m, float l) {
-  if (p.merge) {
-    merge_row<W>(p, t, hd, d, f, m, l);
-  } else if (p.part_o) {
+  if (p.part_o) {
     const int64_t i = (int64_t)part * p.T * p.Hq + (int64_t)t * p.Hq + hd;
     if (d == 0) p.part_ml[i] = make_float2(m, l);
     if (l != 0.f) {
@@ -107,6 +70,9 @@ __device__ __forceinline__ void store_row(const Params &p, int part, int t, int 
     for (int e = 0; e < W; e += 2) o[e / 2] = __floats2half2_rn(f[e] * inv, f[e + 1] * inv);
   }
 }
+
+// Tensor maps of the two caches: boxes of 64 columns of `piece` slots of a page.
+int cache_maps(const Params &p, int hkv, CUtensorMap *tm);
 
 // Tensor-core form (paged_attention_tc.cu): seq false: rows of the batch against the prefix; true: rows of each
 // sequence against the prefix and its own keys.

@@ -421,22 +421,25 @@ static int launch_tc(const Params &p, const CUtensorMap *tm, dim3 grid, cudaStre
   return check_launch("paged_tc");
 }
 
-int tc_launch(const Params &p, int hkv, bool seq, dim3 grid, cudaStream_t st) {
-  // a dimension of one element may come with any stride: the map gets a legal one
-  auto bytes = [](int64_t n, int64_t stride) { return n > 1 ? (uint64_t)stride * 2 : (uint64_t)16; };
-  CUtensorMap tm[3];
-  {
-    const uint64_t dims[4] = {(uint64_t)p.D, (uint64_t)p.G, (uint64_t)hkv, (uint64_t)p.T};
-    const uint64_t str[3] = {bytes(p.G, p.sq_h), bytes(hkv, p.sq_h * p.G), bytes(p.T, p.sq_t)};
-    const uint32_t box[4] = {64, (uint32_t)p.G, 1, (uint32_t)p.tile_tokens};
-    if (int e = encode_tmap_f16_sw128(&tm[0], p.q, 4, dims, str, box)) return e;
-  }
+// a dimension of one element may come with any stride: the map gets a legal one
+static uint64_t stride_bytes(int64_t n, int64_t stride) { return n > 1 ? (uint64_t)stride * 2 : (uint64_t)16; }
+
+int cache_maps(const Params &p, int hkv, CUtensorMap *tm) {
   const uint64_t dims[4] = {(uint64_t)p.D, (uint64_t)hkv, (uint64_t)p.page_size, (uint64_t)p.num_pages};
   const uint32_t box[4] = {64, 1, (uint32_t)p.piece, 1};
-  const uint64_t sk[3] = {bytes(hkv, p.sk_h), bytes(p.page_size, p.sk_s), bytes(p.num_pages, p.sk_p)};
-  const uint64_t sv[3] = {bytes(hkv, p.sv_h), bytes(p.page_size, p.sv_s), bytes(p.num_pages, p.sv_p)};
-  if (int e = encode_tmap_f16_sw128(&tm[1], p.k, 4, dims, sk, box)) return e;
-  if (int e = encode_tmap_f16_sw128(&tm[2], p.v, 4, dims, sv, box)) return e;
+  const uint64_t sk[3] = {stride_bytes(hkv, p.sk_h), stride_bytes(p.page_size, p.sk_s), stride_bytes(p.num_pages, p.sk_p)};
+  const uint64_t sv[3] = {stride_bytes(hkv, p.sv_h), stride_bytes(p.page_size, p.sv_s), stride_bytes(p.num_pages, p.sv_p)};
+  if (int e = encode_tmap_f16_sw128(&tm[0], p.k, 4, dims, sk, box)) return e;
+  return encode_tmap_f16_sw128(&tm[1], p.v, 4, dims, sv, box);
+}
+
+int tc_launch(const Params &p, int hkv, bool seq, dim3 grid, cudaStream_t st) {
+  CUtensorMap tm[3];
+  const uint64_t dims[4] = {(uint64_t)p.D, (uint64_t)p.G, (uint64_t)hkv, (uint64_t)p.T};
+  const uint64_t str[3] = {stride_bytes(p.G, p.sq_h), stride_bytes(hkv, p.sq_h * p.G), stride_bytes(p.T, p.sq_t)};
+  const uint32_t box[4] = {64, (uint32_t)p.G, 1, (uint32_t)p.tile_tokens};
+  if (int e = encode_tmap_f16_sw128(&tm[0], p.q, 4, dims, str, box)) return e;
+  if (int e = cache_maps(p, hkv, tm + 1)) return e;
   if (p.D == 64) return seq ? launch_tc<64, true>(p, tm, grid, st) : launch_tc<64, false>(p, tm, grid, st);
   return seq ? launch_tc<128, true>(p, tm, grid, st) : launch_tc<128, false>(p, tm, grid, st);
 }
