@@ -727,6 +727,7 @@ struct Plan {
   bool stream;                    // the stream of key blocks: own keys, and the prefix unless tc_prefix
   bool stream_prefix;
   int prefix_parts, own_parts;    // slots
+  int cluster;                    // key ranges of a prefix tile that join in a cluster
   int rw;
   int64_t ctas;                   // of the stream
   bool tma;                       // the stream's blocks by TMA
@@ -765,8 +766,9 @@ static Plan make_plan(const hexb_paged_attention_desc *d, int sm_count) {
   if (d->prefix_len > 0 && tc_ok && d->T * G >= 64) {
     pl.tc_prefix = true;
     const int64_t tiles = (int64_t)ceil_div(d->T, pl.tile_tokens) * d->Hkv;
-    const int64_t parts = clamp64(2 * sm_count / tiles, 1, clamp64((pblocks + 1) / 2, 1, 64));
-    pl.prefix_parts = ceil_div(pblocks, ceil_div(pblocks, parts));
+    const int64_t ranges = clamp64(2 * sm_count / tiles, 1, clamp64((pblocks + 1) / 2, 1, 64));
+    for (pl.cluster = 8; pl.cluster > ranges;) pl.cluster /= 2;
+    pl.prefix_parts = (int)(ranges / pl.cluster);
   }
   pl.stream_prefix = d->prefix_len > 0 && !pl.tc_prefix;
   pl.stream = pl.stream_prefix || capacity > 0;
@@ -894,6 +896,7 @@ extern "C" int hexb_paged_attention_f16(const hexb_paged_attention_desc *d, void
   p.scale_log2 = d->sm_scale * 1.44269504f;
   p.tile_tokens = pl.tile_tokens;
   p.piece = pl.piece;
+  p.cluster = pl.cluster;
   if (need) {
     const size_t rows = (size_t)d->T * d->Hq, n = (size_t)pl.parts() * rows;
     uint8_t *w = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~(uintptr_t)15);
@@ -906,7 +909,7 @@ extern "C" int hexb_paged_attention_f16(const hexb_paged_attention_desc *d, void
   cudaStream_t st = (cudaStream_t)stream;
   const int64_t mq = d->max_q > 0 ? d->max_q : paged::ceil_div(d->T, d->B);
   if (pl.seq || pl.tc_prefix) {
-    const int64_t x = paged::ceil_div(pl.seq ? mq : d->T, pl.tile_tokens), y = (int64_t)pl.prefix_parts * (pl.seq ? d->B : 1);
+    const int64_t x = paged::ceil_div(pl.seq ? mq : d->T, pl.tile_tokens), y = (int64_t)pl.prefix_parts * (pl.seq ? d->B : pl.cluster);
     if (y > 65535) return HEXB_ERR_UNSUPPORTED;
     if (int e = paged::tc_launch(p, (int)d->Hkv, pl.seq, dim3((unsigned)x, (unsigned)y, (unsigned)d->Hkv), st)) return e;
   }

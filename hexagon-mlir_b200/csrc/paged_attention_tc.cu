@@ -32,6 +32,17 @@ struct TcCfg {
   static constexpr int TMEM_COLS = 256, O_COL = 128;                      // S0 [0,64), S1 [64,128), O [128,128+HD)
 };
 
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
 // What a tile's key axis consists of: prefix blocks, then own blocks.
 struct Axis {
   int prefix_blocks, lo, hi;   // blocks [lo, hi) of this part
@@ -118,7 +129,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   } else {
     ntok = tokens_used(p);
     part = blockIdx.y;
-    parts = p.prefix_parts;
+    parts = gridDim.y;
   }
   const int tiles = (ntok + TB - 1) / TB;
   // keys of the sequence's own that the tile's last token sees
@@ -263,6 +274,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const int rt = r / p.G, rg = r - rt * p.G;      // token in the tile, query head in the group
     uint32_t it = 0, t = 0;
     bool ok = true;
+    float m_last = -INFINITY, l_last = 0.f;         // of the one tile of a CTA in a cluster
     const float2 mul2 = make_float2(p.scale_log2, p.scale_log2);
     for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
       const Axis a = axis(tile);
@@ -346,6 +358,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         if (lane == 0) tc::mbar_arrive(p_full(b));
       }
       if (!ok) break;
+      if (!SEQ && p.cluster > 1) {                  // joined with the other CTAs of the cluster below
+        if (a.lo < a.hi) {
+          ok = tc::mbar_wait(o_full, 0, abort_flag);
+          tc::tc_fence_after();
+          m_last = m_ref;
+          l_last = ok ? l : 0.f;
+        }
+        break;
+      }
       if (a.lo >= a.hi) {                           // no key for this tile: nothing went through the pipeline
         if (row_ok) {
           float zero[4] = {0.f, 0.f, 0.f, 0.f};
@@ -392,8 +413,66 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         }
       }
     }
+    if (!SEQ && p.cluster > 1) {
+      // The CTAs of a cluster hold the same rows against neighbouring key ranges.  Their parts meet in distributed shared
+      // memory, each CTA adding up its share of the rows: the parts that reach memory, and the join kernel, are
+      // fewer by the cluster's size (16 parts of 2048 rows through memory cost the join 10 us).
+      const int cl = p.cluster, rank = (int)tc::cluster_ctarank();
+      float2 *ml = reinterpret_cast<float2 *>(smem);                          // over Q: the last product has read it
+      const uint32_t so = sK0;                                                // over K and V: [128 rows][HD], 16-byte pieces
+      ml[r] = make_float2(m_last, l_last);                                    // of row r at (piece ^ r)
+      tc::cluster_sync_all();
+      float mm = -INFINITY;
+      const uint32_t mine = tc::smem_u32(&ml[r]);
+      for (int i = 0; i < cl; ++i) {
+        const float2 v = ld_cluster_f2(tc::map_to_rank(mine, (uint32_t)i));
+        if (v.y != 0.f) mm = fmaxf(mm, v.x);
+      }
+      const float alpha = l_last == 0.f ? 0.f : ex2_approx(m_last - mm);
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t o[32];
+        tc::tmem_ld_32x32(tO + lane_off + (uint32_t)(c * 32), o);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          const uint32_t piece = (uint32_t)(c * 8 + g) ^ (uint32_t)(r & (HD / 4 - 1));
+          const bool use = l_last != 0.f;
+          *reinterpret_cast<float4 *>(smem + (so - sQ) + r * HD * 4 + piece * 16) =
+              make_float4(use ? alpha * __uint_as_float(o[g * 4]) : 0.f, use ? alpha * __uint_as_float(o[g * 4 + 1]) : 0.f,
+                          use ? alpha * __uint_as_float(o[g * 4 + 2]) : 0.f, use ? alpha * __uint_as_float(o[g * 4 + 3]) : 0.f);
+        }
+      }
+      tc::cluster_sync_all();
+      const int share = 128 / cl, tid = threadIdx.x - 64;
+      for (int i = tid; i < share * (HD / 4); i += 128) {
+        const int rr = rank * share + i / (HD / 4), d = (i % (HD / 4)) * 4;
+        const int idx = (int)blockIdx.x * TB + rr / p.G;
+        if (rr >= rows_tile || idx >= ntok) continue;
+        float m = -INFINITY, ll = 0.f, f[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint32_t mrow = tc::smem_u32(&ml[rr]);
+        const uint32_t orow = so + (uint32_t)(rr * HD * 4) + (((uint32_t)(d / 4) ^ (uint32_t)(rr & (HD / 4 - 1))) * 16);
+        for (int k = 0; k < cl; ++k) {
+          const float2 v = ld_cluster_f2(tc::map_to_rank(mrow, (uint32_t)k));
+          if (v.y != 0.f) m = fmaxf(m, v.x);
+        }
+#pragma unroll 4
+        for (int k = 0; k < cl; ++k) {
+          const float2 v = ld_cluster_f2(tc::map_to_rank(mrow, (uint32_t)k));
+          ll += v.y == 0.f ? 0.f : v.y * ex2_approx(v.x - m);
+          const float4 q = ld_cluster_f4(tc::map_to_rank(orow, (uint32_t)k));
+          f[0] += q.x; f[1] += q.y; f[2] += q.z; f[3] += q.w;
+        }
+        store_row<4>(p, part / cl, idx, h * p.G + rr % p.G, d, f, m, ll);
+      }
+      tc::cluster_sync_all();                                                 // no CTA leaves while its memory is read
+    }
   }
 
+  if (!SEQ && p.cluster > 1 && warp < 2) {          // the other side of the cluster's barriers
+    __syncwarp();
+    for (int i = 0; i < 3; ++i) tc::cluster_sync_all();
+  }
   // ------------------------------------------------------------ teardown
   if (*abort_flag) {
     for (int i = 0; i < 200; ++i) __nanosleep(1000);  // lets copies in flight land before the CTA's memory goes
@@ -417,7 +496,26 @@ static int launch_tc(const Params &p, const CUtensorMap *tm, dim3 grid, cudaStre
     HEXB_CUDA_OK(cudaFuncSetAttribute(paged_tc_kernel<HD, SEQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<HD>::SMEM));
     once.mark(dev);
   }
-  HEXB_CUDA_OK(launch_pdl(paged_tc_kernel<HD, SEQ>, grid, dim3(192), (size_t)TcCfg<HD>::SMEM, st, tm[0], tm[1], tm[2], p));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = TcCfg<HD>::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (option(OPT_pdl, 1)) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (!SEQ && p.cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = 1;
+    attr[n].val.clusterDim.y = (unsigned)p.cluster;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  HEXB_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_tc_kernel<HD, SEQ>, tm[0], tm[1], tm[2], p));
   return check_launch("paged_tc");
 }
 
