@@ -77,127 +77,6 @@ struct RowCfg {
   static constexpr int PER_SM = DP == 64 ? 4 : DP == 128 ? 2 : 1;
 };
 
-// A place in the list of units.
-struct Cursor {
-  int b;                 // -1: the prefix
-  int tok0, ntok, len, nb, nt;
-  int h, tile, j;
-};
-
-template <int RW>
-__device__ __forceinline__ long long sequence_units(const Params &p, int b, int *tok0, int *ntok, int *len) {
-  if (b < 0) {
-    *tok0 = 0;
-    *ntok = tokens_used(p);
-    *len = p.prefix_len;
-  } else {
-    seq_range(p, b, *tok0, *ntok);
-    *len = seq_len(p, b);
-  }
-  // a tile without keys is one unit too: its rows get an empty part
-  return (long long)((*ntok * p.G + 16 * RW - 1) / (16 * RW)) * (p.Hq / p.G) * max((*len + 63) / 64, 1);
-}
-
-template <int RW>
-__device__ __forceinline__ void enter(const Params &p, Cursor &c) {
-  // the next sequence from c.b on that has tokens
-  for (; c.b < p.nseq; ++c.b) {
-    if (sequence_units<RW>(p, c.b, &c.tok0, &c.ntok, &c.len) > 0) break;
-  }
-  c.nb = max((c.len + 63) / 64, 1);
-  c.nt = (c.ntok * p.G + 16 * RW - 1) / (16 * RW);
-}
-
-template <int RW>
-__device__ __forceinline__ void advance(const Params &p, Cursor &c) {
-  if (++c.j < c.nb) return;
-  c.j = 0;
-  if (++c.tile < c.nt) return;
-  c.tile = 0;
-  if (++c.h < p.Hq / p.G) return;
-  c.h = 0;
-  ++c.b;
-  enter<RW>(p, c);
-}
-
-// Keys [0, end) of the cursor's sequence are seen by some row of its tile.
-template <int RW>
-__device__ __forceinline__ int end_of(const Params &p, const Cursor &c) {
-  if (c.b < 0) return c.len;
-  return min(c.len, c.len - c.ntok + min(c.ntok - 1, (c.tile * 16 * RW + 16 * RW - 1) / p.G) + 1);
-}
-
-// This CTA's stretch of the list: units [start, stop), `per` units a CTA, the cursor at start.  All NT threads call it.
-template <int RW, int NT>
-__device__ __forceinline__ void find_stretch(const Params &p, long long &start, long long &stop, long long &per, Cursor &c) {
-  constexpr int NW = NT / 32;
-  __shared__ long long s_sum[NW];
-  __shared__ int s_max[NW];
-  __shared__ int s_b;
-  __shared__ long long s_off;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int first_b = p.stream_prefix ? -1 : 0;
-  long long total = 0;
-  int longest = 0;
-  for (int b = first_b + tid; b < p.nseq; b += NT) {
-    int t0, n, len;
-    const long long u = sequence_units<RW>(p, b, &t0, &n, &len);
-    total += u;
-    // blocks that one part slot has to cover at least, so that a tile's runs fit its slots
-    const int slots = (b < 0 ? p.prefix_parts : p.own_parts) - 1;
-    if (u) longest = max(longest, slots > 0 ? ((len + 63) / 64 + slots - 1) / slots : (len + 63) / 64);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-  }
-  if (lane == 0) {
-    s_sum[warp] = total;
-    s_max[warp] = longest;
-  }
-  __syncthreads();
-  total = 0;
-  for (int w = 0; w < NW; ++w) {
-    total += s_sum[w];
-    longest = max(longest, s_max[w]);
-  }
-  per = max((total + gridDim.x - 1) / gridDim.x, (long long)max(longest, 1));
-  start = blockIdx.x * per;
-  stop = min(start + per, total);
-  if (start >= stop) return;
-  long long base = 0;
-  for (int b0 = first_b; b0 < p.nseq; b0 += NT) {
-    int t0, n, len;
-    const long long u = b0 + tid < p.nseq ? sequence_units<RW>(p, b0 + tid, &t0, &n, &len) : 0;
-    long long incl = u;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    __syncthreads();
-    if (lane == 31) s_sum[warp] = incl;
-    if (tid == 0) s_b = p.nseq;
-    __syncthreads();
-    long long excl = base + incl - u;
-    for (int w = 0; w < warp; ++w) excl += s_sum[w];
-    if (start >= excl && start < excl + u) {
-      s_b = b0 + tid;
-      s_off = start - excl;
-    }
-    for (int w = 0; w < NW; ++w) base += s_sum[w];
-    __syncthreads();
-    if (s_b < p.nseq) break;
-  }
-  c.b = s_b;
-  enter<RW>(p, c);
-  const int off = (int)(s_off % ((long long)c.nb * c.nt)), tile_head = off / c.nb;
-  c.h = (int)(s_off / ((long long)c.nb * c.nt));
-  c.j = off - tile_head * c.nb;
-  c.tile = tile_head;
-}
-
 // The running state of one tile in the consumer warps.
 template <int DP, int RW>
 struct Run {
@@ -208,10 +87,12 @@ struct Run {
   int tok[2], head[2];
   bool row_ok[2];
   int lane, rw, kw;
+  int first_j;            // block the run began with
 
   // fragments of Q: rows g and g + 8 of this warp's 16
   __device__ __forceinline__ void begin(const Params &p, const Cursor &c) {
     const int row0 = c.tile * ROWS, rows = c.ntok * p.G;
+    first_j = c.j;
     const __half *q[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -328,17 +209,14 @@ struct Run {
     }
   }
 
-  // The run is over: its part.  Runs of a tile are numbered by the CTAs that hold them.  All 128 consumer threads.
+  // The run is over: its part, or the output itself.  All 128 consumer threads.
   __device__ __forceinline__ void end(const Params &p, const Cursor &c, long long unit, long long per, float *xch) {
-    const long long tile_first = unit - c.j;
-    const int run = (int)((long long)blockIdx.x - tile_first / per);
-    const int part = (c.b < 0 ? 0 : p.prefix_parts) + run;
-    int *runs = c.b < 0 ? p.prefix_runs : p.own_runs;
+    const RunPlace place(p, c, first_j, c.j + 1, unit - c.j, per, ROWS);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-      if (c.j == c.nb - 1 && runs && kw == 0 && (lane & 3) == 0 && row_ok[i]) runs[(int64_t)tok[i] * p.Hq + head[i]] = run + 1;
+      if (kw == 0 && (lane & 3) == 0 && row_ok[i]) place.describe(p, c, tok[i], head[i], rw * 16 + (lane >> 2) + 8 * i);
     }
     if (KW > 1) {
       // Join the key groups of a row group.  All scale to their common maximum; then key group w collects columns
@@ -422,7 +300,7 @@ struct Run {
           for (int n = 0; n < PN; ++n) {
             const int d = kw * QC + pc * PC + n * 8 + (lane & 3) * 2;
             float v[2] = {f[n][2 * i], f[n][2 * i + 1]};
-            if (d < p.D) store_row<2>(p, part, tok[i], head[i], d, v, mm[i], ll[i]);
+            if (d < p.D) store_row<2>(p, place.index(p, tok[i], head[i], r0 + 8 * i), tok[i], head[i], d, v, mm[i], ll[i]);
           }
         }
       }
@@ -434,7 +312,7 @@ struct Run {
         for (int n = 0; n < DP / 8; ++n) {
           const int d = n * 8 + (lane & 3) * 2;
           float f[2] = {o[n][2 * i], o[n][2 * i + 1]};
-          if (d < p.D) store_row<2>(p, part, tok[i], head[i], d, f, m[i], l[i]);
+          if (d < p.D) store_row<2>(p, place.index(p, tok[i], head[i], rw * 16 + (lane >> 2) + 8 * i), tok[i], head[i], d, f, m[i], l[i]);
         }
       }
     }
@@ -471,7 +349,7 @@ paged_stream_tma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
   if (!p.follows_prefix) pdl_wait();
   long long start, stop, per;
   Cursor c;
-  find_stretch<RW, 160>(p, start, stop, per, c);   // its barriers also publish the ones set up above
+  find_stretch<160>(p, 16 * RW, start, stop, per, c);   // its barriers also publish the ones set up above
   if (start < stop) {
     const int units = (int)(stop - start);
     if (warp == 4) {
@@ -481,7 +359,7 @@ paged_stream_tma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
         slot = 0;
         if (lane < pieces && u < units) {
           const int key = c.j * BN + lane * p.piece;
-          if (key < end_of<RW>(p, c)) {
+          if (key < end_of(p, 16 * RW, c)) {
             const int pi = key / p.page_size;
             slot = key - pi * p.page_size;
             const int got = c.b < 0 ? p.prefix_pages[pi] : p.table[(int64_t)c.b * p.table_stride + pi];
@@ -494,7 +372,7 @@ paged_stream_tma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
       int slot_next, page_next = lookup(0, slot_next);
       for (int u = 0; u < units; ++u) {
         const int st = u % ST, page = page_next, slot = slot_next, h = c.h;
-        if (u + 1 < units) advance<RW>(p, c);
+        if (u + 1 < units) advance(p, 16 * RW, c);
         page_next = lookup(u + 1, slot_next);
         if (!tc::mbar_wait(empty(st), (uint32_t)(u / ST + 1) & 1u, abort_flag)) break;
         if (lane == 0) tc::mbar_arrive_expect_tx(full(st), 2 * cfg::KV);
@@ -518,7 +396,7 @@ paged_stream_tma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
       for (int u = 0; u < units; ++u) {
         if (u == 0 || c.j == 0) {
           r.begin(p, c);
-          end = end_of<RW>(p, c);
+          end = end_of(p, 16 * RW, c);
         }
         const int st = u % ST;
         const uint32_t sk = s0 + (uint32_t)st * 2 * cfg::KV, sv = sk + cfg::KV;
@@ -542,7 +420,7 @@ paged_stream_tma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(empty(st));
         if (c.j == c.nb - 1 || u == units - 1) r.end(p, c, start + u, per, xch);
-        if (u + 1 < units) advance<RW>(p, c);
+        if (u + 1 < units) advance(p, 16 * RW, c);
       }
     }
     if (*abort_flag) {
@@ -568,7 +446,7 @@ paged_stream_kernel(const Params p) {
   if (!p.follows_prefix) pdl_wait();
   long long start, stop, per;
   Cursor cc, cl;                        // the unit being computed, the one whose pages are looked up
-  find_stretch<RW, THREADS>(p, start, stop, per, cc);
+  find_stretch<THREADS>(p, 16 * RW, start, stop, per, cc);
   if (start < stop) {
     const int units = (int)(stop - start);
     int looked = 0, fetched = 0;
@@ -577,7 +455,7 @@ paged_stream_kernel(const Params p) {
       int page = -1;
       if (looked < units && tid < BN) {
         const int key = cl.j * BN + tid;
-        if (key < end_of<RW>(p, cl)) {
+        if (key < end_of(p, 16 * RW, cl)) {
           const int pi = key / p.page_size;
           page = cl.b < 0 ? p.prefix_pages[pi] : p.table[(int64_t)cl.b * p.table_stride + pi];
         }
@@ -589,7 +467,7 @@ paged_stream_kernel(const Params p) {
         if (tid < BN) {
           const int key = cl.j * BN + tid;
           int64_t ko = -1, vo = -1;
-          if (key < end_of<RW>(p, cl)) {
+          if (key < end_of(p, 16 * RW, cl)) {
             if ((unsigned)page < (unsigned)p.num_pages) {
               const int64_t in = key % p.page_size;
               ko = (int64_t)page * p.sk_p + in * p.sk_s + (int64_t)cl.h * p.sk_h;
@@ -602,7 +480,7 @@ paged_stream_kernel(const Params p) {
           o[tid] = ko;
           o[BN + tid] = vo;
         }
-        advance<RW>(p, cl);
+        advance(p, 16 * RW, cl);
       }
       ++looked;
     };
@@ -643,7 +521,7 @@ paged_stream_kernel(const Params p) {
     for (int u = 0; u < units; ++u) {
       if (u == 0 || cc.j == 0) {
         r.begin(p, cc);
-        end = end_of<RW>(p, cc);
+        end = end_of(p, 16 * RW, cc);
       }
       cp_async_wait<1>();
       __syncthreads();  // unit u landed for all; unit u - 1's readers are done; offsets of u + 2 are visible
@@ -653,7 +531,7 @@ paged_stream_kernel(const Params p) {
       r.step(p, cc, end, sk, sk + cfg::KV);
       publish(page_next);
       if (cc.j == cc.nb - 1 || u == units - 1) r.end(p, cc, start + u, per, reinterpret_cast<float *>(smem + cfg::XCH));
-      if (u + 1 < units) advance<RW>(p, cc);
+      if (u + 1 < units) advance(p, 16 * RW, cc);
     }
     cp_async_wait<0>();
   }
@@ -672,14 +550,30 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const Params p) {
   const int t = (int)(row / p.Hq), hd = (int)(row - (int64_t)t * p.Hq);
   if (t >= tokens_used(p)) return;
   const int64_t n = (int64_t)p.T * p.Hq;
-  // the parts of a row: those of the prefix, then those of its own keys; each side may hold fewer runs than slots
-  const int np = p.prefix_runs ? min(max(p.prefix_runs[row], 0), p.prefix_parts) : p.prefix_parts;
-  const int no = p.own_runs ? min(max(p.own_runs[row], 0), p.own_parts) : p.own_parts;
+  // The parts of a row: those of the prefix, then those of its own keys; each side either in row order, or the runs of
+  // its tile where their CTAs left them.
+  auto side = [&](const int4 *desc, int dense, int &cta, int &r) {
+    if (!desc) return dense;
+    const int4 v = desc[row];    // (rows that belong to no sequence have none: whatever is there stays in bounds)
+    cta = min(max(v.y, 0), p.ctas - 1);
+    r = min(max(v.z, 0), p.tile_rows - 1);
+    return min(max(v.x, -1), p.ctas - cta);
+  };
+  int pc = 0, pr = 0, oc = 0, orow = 0;
+  int np = side(p.prefix_desc, p.prefix_desc ? 0 : p.prefix_parts, pc, pr), no = side(p.own_desc, 0, oc, orow);
+  if (np < 0 || no < 0) return;  // stored by its one run
+  const bool pcut = p.prefix_desc && np > 0, ocut = no > 0;
+  if (p.prefix_desc && np == 0) np = 1;
+  if (p.own_desc && no == 0) no = 1;
   const int parts = np + no;
-  auto slot = [&](int i) { return i < np ? i : p.prefix_parts + i - np; };
+  auto slot = [&](int i) -> int64_t {
+    if (i < np) return pcut ? p.run_base + ((int64_t)(pc + i) * 2 + (i == 0)) * p.tile_rows + pr : i * n + row;
+    i -= np;
+    return ocut ? p.run_base + ((int64_t)(oc + i) * 2 + (i == 0)) * p.tile_rows + orow : p.own_slot * n + row;
+  };
   float mm = -INFINITY;
   for (int i = lane; i < parts; i += 32) {
-    const float2 ml = p.part_ml[slot(i) * n + row];
+    const float2 ml = p.part_ml[slot(i)];
     if (ml.y != 0.f) mm = fmaxf(mm, ml.x);
   }
   mm = warp_max(mm);
@@ -688,7 +582,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const Params p) {
     float f[4] = {0.f, 0.f, 0.f, 0.f}, ll = 0.f;
     for (int i0 = 0; i0 < parts; i0 += 32) {
       float2 ml = make_float2(0.f, 0.f);
-      if (i0 + lane < parts) ml = p.part_ml[slot(i0 + lane) * n + row];
+      if (i0 + lane < parts) ml = p.part_ml[slot(i0 + lane)];
       const float w = ml.y == 0.f ? 0.f : exp2f(ml.x - mm);  // no key seen: no O either
       ll += warp_sum(w * ml.y);
       const int m = min(32, parts - i0);
@@ -697,7 +591,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const Params p) {
         // every lane loads, from a slot in bounds, and then selects: loads behind a branch would not overlap
         const int k = i + sub;
         const float a = __shfl_sync(0xffffffffu, w, k & 31);
-        const float4 v = __ldcs(reinterpret_cast<const float4 *>(p.part_o + (slot(i0 + min(k, m - 1)) * n + row) * p.D + min(d, p.D - 4)));
+        const float4 v = __ldcs(reinterpret_cast<const float4 *>(p.part_o + slot(i0 + min(k, m - 1)) * p.D + min(d, p.D - 4)));
         const bool use = k < m && a != 0.f;
         f[0] = fmaf(use ? a : 0.f, use ? v.x : 0.f, f[0]);
         f[1] = fmaf(use ? a : 0.f, use ? v.y : 0.f, f[1]);
@@ -724,15 +618,14 @@ static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // How a call is cut.  A function of the sizes alone, so that the workspace query and the launch agree.
 struct Plan {
   bool seq, tc_prefix;            // tensor-core forms
-  bool stream;                    // the stream of key blocks: own keys, and the prefix unless tc_prefix
-  bool stream_prefix;
-  int prefix_parts, own_parts;    // slots
+  bool stream, stream_prefix;     // the stream of key blocks: own keys, and the prefix unless tc_prefix
+  bool tma;                       // its blocks by TMA
+  bool join;                      // some row may have more than one part
+  int prefix_parts;               // parts in row order that the prefix leaves
   int cluster;                    // key ranges of a prefix tile that join in a cluster
-  int rw;
-  int64_t ctas;                   // of the stream
-  bool tma;                       // the stream's blocks by TMA
-  int tile_tokens, piece;
-  int parts() const { return prefix_parts + own_parts; }
+  int slots;                      // parts in row order, prefix and own
+  int rw, tile_rows, tile_tokens, piece;
+  int64_t ctas;                   // of the launch that walks the list of units
 };
 
 static int rw_for(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
@@ -744,8 +637,8 @@ static Plan make_plan(const hexb_paged_attention_desc *d, int sm_count) {
   const int64_t mq = d->max_q > 0 ? d->max_q : ceil_div(d->T, d->B);
   const int64_t pblocks = ceil_div(d->prefix_len, 64), oblocks = ceil_div(capacity, 64);
   // What TMA can address: page pieces of at least the 8 rows of a swizzle atom, no stride of 0.
-  // The tensor-core forms want besides: a positive scale, and enough rows to fill half of a 128-row tile; below that the key stream, not the products, is
-  // what takes the time, and the small tiles of mma.sync read it as fast.
+  // The tensor-core forms want besides: a positive scale, and enough rows to fill half of a 128-row tile; below that the
+  // key stream, not the products, is what takes the time, and the small tiles of mma.sync read it as fast.
   pl.piece = (int)(d->page_size & -d->page_size);
   if (pl.piece > 64) pl.piece = 64;
   bool tma_ok = (d->D == 64 || d->D == 128) && pl.piece >= 8;
@@ -755,14 +648,17 @@ static Plan make_plan(const hexb_paged_attention_desc *d, int sm_count) {
   pl.tma = tma_ok;
   const bool tc_ok = tma_ok && fits(0) && fits(1) && d->sm_scale > 0.f && G <= 128 && (d->Hkv <= 1 || d->strides[1] * G < ((int64_t)1 << 38));
   pl.tile_tokens = tc_ok ? (int)(128 / G) : 0;
+  // CTAs for a list of at most `tiles` tiles of at most `blocks` blocks: those that fit the GPU, fewer for a short list
+  auto ctas_for = [&](double units, int64_t fit) { return clamp64(units < (double)fit ? (int64_t)units : fit, 1, fit); };
   if (tc_ok && mq * G >= 64 && capacity > 0) {
-    // tiles of one sequence each, over prefix and own keys: cut the axis only when the tiles leave SMs idle
+    // tiles of one sequence each, over the prefix and its own keys
     pl.seq = true;
-    const int64_t tiles = d->B * ceil_div(mq, pl.tile_tokens) * d->Hkv;
-    pl.prefix_parts = (int)clamp64(2 * sm_count / tiles, 1, clamp64((pblocks + oblocks) / 8, 1, 32));
+    pl.tile_rows = 128;
+    const double tiles = (double)(ceil_div(d->T, pl.tile_tokens) + d->B) * d->Hkv;
+    pl.ctas = ctas_for(tiles * (pblocks + oblocks), 2 * sm_count);
+    pl.join = pblocks + oblocks > 1;
     return pl;
   }
-  const int per_sm = d->D <= 64 ? 4 : d->D <= 128 ? 2 : 1;
   if (d->prefix_len > 0 && tc_ok && d->T * G >= 64) {
     pl.tc_prefix = true;
     const int64_t tiles = (int64_t)ceil_div(d->T, pl.tile_tokens) * d->Hkv;
@@ -773,29 +669,28 @@ static Plan make_plan(const hexb_paged_attention_desc *d, int sm_count) {
   pl.stream_prefix = d->prefix_len > 0 && !pl.tc_prefix;
   pl.stream = pl.stream_prefix || capacity > 0;
   if (pl.stream) {
+    const int per_sm = d->D <= 64 ? 4 : d->D <= 128 ? 2 : 1;
     pl.rw = rw_for(mq * G);
     if ((pl.stream_prefix && d->T * G > 128) || d->D > 128) pl.rw = 4;
-    const int64_t rows = 16 * pl.rw;
-    const int64_t fit = (int64_t)sm_count * per_sm;
-    // units at most (a tile of every sequence may be cut short), so that a small call launches no idle CTA
-    const int64_t ptiles = pl.stream_prefix ? ceil_div(d->T * G, rows) * d->Hkv : 0;
-    const int64_t otiles = (ceil_div(d->T * G, rows) + d->B) * d->Hkv;
-    const double most = (double)ptiles * pblocks + (double)otiles * (oblocks > 1 ? oblocks : 1);
-    pl.ctas = most < (double)fit ? (int64_t)most : fit;
-    if (pl.ctas < 1) pl.ctas = 1;
-    // Slots for the runs of a tile: twice its share of the CTAs (ragged lengths); if some tile is longer still, the
-    // kernel gives every CTA so many units that its runs fit.
-    const int64_t tiles = ptiles + (capacity > 0 ? d->B * ceil_div(mq * G, rows) * d->Hkv : 0);
-    const int64_t slots = clamp64(2 + 2 * pl.ctas / tiles, 3, 64);
-    if (pl.stream_prefix) pl.prefix_parts = (int)clamp64(pblocks, 1, slots);
-    if (capacity > 0) pl.own_parts = (int)clamp64(oblocks, 1, slots);
+    pl.tile_rows = 16 * pl.rw;
+    const double ptiles = pl.stream_prefix ? (double)ceil_div(d->T * G, pl.tile_rows) * d->Hkv : 0.;
+    const double otiles = capacity > 0 ? (double)(ceil_div(d->T * G, pl.tile_rows) + d->B) * d->Hkv : 0.;
+    pl.ctas = ctas_for(ptiles * pblocks + otiles * (oblocks > 1 ? oblocks : 1), (int64_t)sm_count * per_sm);
   }
+  const int sides = (d->prefix_len > 0) + (capacity > 0);
+  pl.join = sides != 1 || (pl.tc_prefix ? pl.prefix_parts > 1 : pblocks + oblocks > 1);
+  if (pl.tc_prefix) pl.slots = pl.prefix_parts > 1 || sides > 1 ? pl.prefix_parts : 0;
+  else if (pl.stream_prefix && sides > 1) pl.slots = 1;
+  if (sides > 1) ++pl.slots;      // own keys of tiles that were not cut
   return pl;
 }
 
+static size_t parts_of(const hexb_paged_attention_desc *d, const Plan &pl) {
+  return (size_t)pl.slots * d->T * d->Hq + (pl.tile_rows ? (size_t)pl.ctas * 2 * pl.tile_rows : 0);
+}
 static size_t ws_need(const hexb_paged_attention_desc *d, const Plan &pl) {
-  if (pl.parts() < 2) return 0;
-  return (size_t)pl.parts() * d->T * d->Hq * ((size_t)d->D * 4 + 8) + (size_t)d->T * d->Hq * 8 + 256;
+  if (!pl.join || !parts_of(d, pl)) return 0;
+  return parts_of(d, pl) * ((size_t)d->D * 4 + 8) + (size_t)d->T * d->Hq * 2 * sizeof(int4) + 256;
 }
 
 template <int DP, int RW>
@@ -891,27 +786,34 @@ extern "C" int hexb_paged_attention_f16(const hexb_paged_attention_desc *d, void
   p.T = (int)d->T; p.B = (int)d->B; p.Hq = (int)d->Hq; p.G = (int)(d->Hq / d->Hkv); p.D = (int)d->D;
   p.prefix_len = (int)d->prefix_len; p.page_size = (int)d->page_size; p.num_pages = (int)d->num_pages;
   p.own_capacity = (int)(d->table_width * d->page_size);
-  p.prefix_parts = pl.prefix_parts; p.own_parts = pl.own_parts;
+  p.prefix_parts = pl.prefix_parts;
   p.nseq = p.own_capacity ? p.B : 0;
   p.scale_log2 = d->sm_scale * 1.44269504f;
   p.tile_tokens = pl.tile_tokens;
   p.piece = pl.piece;
   p.cluster = pl.cluster;
+  p.ctas = (int)pl.ctas;
+  p.tile_rows = pl.tile_rows;
+  const bool both = d->prefix_len > 0 && p.own_capacity > 0 && !pl.seq;
+  p.prefix_slot = pl.stream_prefix && both ? 0 : -1;
+  p.own_slot = both ? pl.slots - 1 : -1;
   if (need) {
-    const size_t rows = (size_t)d->T * d->Hq, n = (size_t)pl.parts() * rows;
+    const size_t rows = (size_t)d->T * d->Hq, n = parts_of(d, pl);
     uint8_t *w = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~(uintptr_t)15);
     p.part_o = reinterpret_cast<float *>(w);
     p.part_ml = reinterpret_cast<float2 *>(w + n * d->D * 4);
-    int *runs = reinterpret_cast<int *>(w + n * (d->D * 4 + 8));
-    if (pl.stream_prefix) p.prefix_runs = runs;
-    if (pl.own_parts) p.own_runs = runs + rows;
+    p.run_base = (int64_t)pl.slots * rows;
+    int4 *desc = reinterpret_cast<int4 *>(w + (n * (d->D * 4 + 8) + 15) / 16 * 16);
+    if (pl.stream_prefix) p.prefix_desc = desc;
+    if (p.own_capacity) p.own_desc = desc + rows;
   }
   cudaStream_t st = (cudaStream_t)stream;
-  const int64_t mq = d->max_q > 0 ? d->max_q : paged::ceil_div(d->T, d->B);
-  if (pl.seq || pl.tc_prefix) {
-    const int64_t x = paged::ceil_div(pl.seq ? mq : d->T, pl.tile_tokens), y = (int64_t)pl.prefix_parts * (pl.seq ? d->B : pl.cluster);
-    if (y > 65535) return HEXB_ERR_UNSUPPORTED;
-    if (int e = paged::tc_launch(p, (int)d->Hkv, pl.seq, dim3((unsigned)x, (unsigned)y, (unsigned)d->Hkv), st)) return e;
+  if (pl.seq) {
+    p.shared_blocks = paged::ceil_div(d->prefix_len, 64);
+    if (int e = paged::tc_launch(p, (int)d->Hkv, true, dim3((unsigned)pl.ctas), st)) return e;
+  } else if (pl.tc_prefix) {
+    const dim3 grid((unsigned)paged::ceil_div(d->T, pl.tile_tokens), (unsigned)(pl.prefix_parts * pl.cluster), (unsigned)d->Hkv);
+    if (int e = paged::tc_launch(p, (int)d->Hkv, false, grid, st)) return e;
   }
   if (pl.stream) {
     p.follows_prefix = pl.tc_prefix;
@@ -921,7 +823,7 @@ extern "C" int hexb_paged_attention_f16(const hexb_paged_attention_desc *d, void
       if (int e = paged::cache_maps(p, (int)d->Hkv, tm)) return e;
     if (int e = paged::dispatch_stream(p, pl.rw, pl.tma ? tm : nullptr, dim3((unsigned)pl.ctas), st)) return e;
   }
-  if (pl.parts() != 1) {
+  if (pl.join) {
     // also the call without any key: its rows are set to zero
     const dim3 grid((unsigned)((d->T * d->Hq + 3) / 4));
     if (d->D <= 64) HEXB_CUDA_OK(launch_pdl(paged::paged_join_kernel<16>, grid, dim3(128), 0, st, p));

@@ -43,11 +43,6 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t a) {
   return v;
 }
 
-// What a tile's key axis consists of: prefix blocks, then own blocks.
-struct Axis {
-  int prefix_blocks, lo, hi;   // blocks [lo, hi) of this part
-};
-
 template <int HD, bool SEQ>
 __global__ void __launch_bounds__(192, 2)
 paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -73,7 +68,6 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int TB = p.tile_tokens, rows_tile = TB * p.G;
-  const int h = blockIdx.z;
 
   if (threadIdx.x == 0) {
     tc::mbar_init(q_full, 1);
@@ -115,33 +109,50 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   pdl_launch_dependents();
   const uint32_t tO = tmem_base + cfg::O_COL;
 
-  int tok0 = 0, ntok, own = 0, part, parts;
-  const int *own_pages = nullptr;
+  // SEQ: the CTA's stretch of the list of units, segment by segment (the blocks of one tile); else one tile and range.
+  long long u = 0, stop = 1, per = 1;
+  Cursor cur;
+  int part = 0;
   if (SEQ) {
-    const int b = blockIdx.y % p.B;
-    part = blockIdx.y / p.B;
-    parts = p.prefix_parts;   // this form's parts, over the whole axis
-    seq_range(p, b, tok0, ntok);
-    if (p.own_capacity) {
-      own = seq_len(p, b);
-      own_pages = p.table + (int64_t)b * p.table_stride;
-    }
+    find_stretch<192>(p, rows_tile, u, stop, per, cur);
   } else {
-    ntok = tokens_used(p);
+    cur.b = -1;
+    cur.tok0 = 0;
+    cur.ntok = tokens_used(p);
+    cur.len = 0;
+    cur.nb = 1;
+    cur.tile = blockIdx.x;
+    cur.h = blockIdx.z;
+    cur.j = 0;
     part = blockIdx.y;
-    parts = gridDim.y;
+    if (cur.tile * TB >= cur.ntok) stop = 0;
   }
-  const int tiles = (ntok + TB - 1) / TB;
-  // keys of the sequence's own that the tile's last token sees
-  auto own_end = [&](int tile) { return SEQ ? max(0, own - ntok + min((tile + 1) * TB, ntok)) : 0; };
-  auto axis = [&](int tile) {
-    Axis a;
-    a.prefix_blocks = (p.prefix_len + BN - 1) / BN;
-    const int total = a.prefix_blocks + (own_end(tile) + BN - 1) / BN;
-    const int per = (total + parts - 1) / parts;
-    a.lo = min(part * per, total);
-    a.hi = min(a.lo + per, total);
-    return a;
+  const int prefix_blocks = (p.prefix_len + BN - 1) / BN;
+  // The segment at the cursor: units [j0, j1) of its tile, of which [lo, hi) hold keys that some row sees.
+  struct Segment {
+    int j0, j1, lo, hi, own_end;
+  };
+  auto segment = [&]() {
+    Segment s;
+    if (SEQ) {
+      s.own_end = max(0, cur.len - cur.ntok + min((cur.tile + 1) * TB, cur.ntok));
+      s.j0 = cur.j;
+      s.j1 = (int)min((long long)cur.nb, cur.j + (stop - u));
+      s.lo = s.j0;
+      s.hi = min(s.j1, prefix_blocks + (s.own_end + BN - 1) / BN);
+    } else {
+      const int n = (prefix_blocks + (int)gridDim.y - 1) / (int)gridDim.y;
+      s.own_end = 0;
+      s.j0 = 0;
+      s.j1 = 1;
+      s.lo = min(part * n, prefix_blocks);
+      s.hi = min(s.lo + n, prefix_blocks);
+    }
+    return s;
+  };
+  auto next = [&](const Segment &s) {
+    u += s.j1 - s.j0;
+    if (SEQ && u < stop) advance(p, rows_tile, cur, s.j1 - s.j0);
   };
 
   if (warp == 0) {
@@ -149,22 +160,26 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     uint32_t it = 0, t = 0, tails = 0;
     bool ok = true;
     const int pieces = BN / p.piece;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-      const Axis a = axis(tile);
-      if (a.lo >= a.hi) continue;
-      const int oend = own_end(tile);
+    for (; u < stop && ok;) {
+      const Segment a = segment();
+      if (a.lo >= a.hi) {
+        next(a);
+        continue;
+      }
+      const int oend = a.own_end, h = cur.h;
+      const int *own_pages = SEQ ? p.table + (int64_t)cur.b * p.table_stride : nullptr;
       if (t > 0 && !tc::mbar_wait(q_empty, (t - 1u) & 1u, abort_flag)) break;
       ++t;
       if (lane == 0) {
         tc::mbar_arrive_expect_tx(q_full, (uint32_t)rows_tile * HD * 2);
 #pragma unroll
         for (int c = 0; c < cfg::CHUNKS; ++c)
-          tc::tma_load_4d(sQ + c * cfg::Q_CHUNK, &tmQ, c * 64, 0, h, tok0 + tile * TB, q_full);
+          tc::tma_load_4d(sQ + c * cfg::Q_CHUNK, &tmQ, c * 64, 0, h, cur.tok0 + cur.tile * TB, q_full);
       }
       // page of this lane's piece of block j; a piece without keys and a page outside the cache read as zeros
       auto lookup = [&](int j, int &slot) {
-        const bool pre = j < a.prefix_blocks;
-        const int key = (pre ? j : j - a.prefix_blocks) * BN + lane * p.piece;
+        const bool pre = j < prefix_blocks;
+        const int key = (pre ? j : j - prefix_blocks) * BN + lane * p.piece;
         int page = p.num_pages;
         slot = 0;
         if (lane < pieces && j < a.hi && key < (pre ? p.prefix_len : oend)) {
@@ -191,8 +206,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             tc::tma_load_4d(sK0 + b * cfg::KV_BYTES + c * cfg::KV_CHUNK + at, &tmK, c * 64, h, slot, page, k_full(b));
         }
         if (!tc::mbar_wait(v_empty(b), ph ^ 1u, abort_flag)) { ok = false; break; }
-        const bool pre = j < a.prefix_blocks;
-        const int filled = (pre ? p.prefix_len - j * BN : oend - (j - a.prefix_blocks) * BN);  // keys of the block
+        const bool pre = j < prefix_blocks;
+        const int filled = (pre ? p.prefix_len - j * BN : oend - (j - prefix_blocks) * BN);  // keys of the block
         const uint32_t bar = filled < BN ? tail : v_full(b);
         if (lane == 0) tc::mbar_arrive_expect_tx(bar, cfg::KV_BYTES);
         __syncwarp();
@@ -215,6 +230,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           if (lane == 0) tc::mbar_arrive(v_full(b));
         }
       }
+      next(a);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
@@ -239,8 +255,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         if (last) tc::mma_commit(q_empty);
       };
       uint32_t it = 0, t = 0;
-      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-        const Axis a = axis(tile);
+      for (; u < stop && ok;) {
+        const Segment a = segment();
+        next(a);
         if (a.lo >= a.hi) continue;
         if (!tc::mbar_wait(q_full, t & 1u, abort_flag)) break;
         issue_qk(it, a.lo + 1 == a.hi);
@@ -276,13 +293,19 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     bool ok = true;
     float m_last = -INFINITY, l_last = 0.f;         // of the one tile of a CTA in a cluster
     const float2 mul2 = make_float2(p.scale_log2, p.scale_log2);
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-      const Axis a = axis(tile);
-      const int idx = tile * TB + rt;               // token of the sequence (or batch)
-      const bool row_ok = rt < TB && idx < ntok;
-      const int oend = own_end(tile);
-      const int sees = own - ntok + idx + 1;        // own keys this row sees (SEQ)
-      const int64_t row = (int64_t)(tok0 + idx) * p.Hq + h * p.G + rg;
+    for (; u < stop && ok;) {
+      const Segment a = segment();
+      const int idx = cur.tile * TB + rt;           // token of the sequence (or batch)
+      const bool row_ok = rt < TB && idx < cur.ntok;
+      const int sees = cur.len - cur.ntok + idx + 1;   // own keys this row sees (SEQ)
+      const int tok = cur.tok0 + idx, hd = cur.h * p.G + rg;
+      int64_t dest = part < 0 || !p.part_o ? -1 : (int64_t)part * p.T * p.Hq + (int64_t)tok * p.Hq + hd;
+      if (SEQ) {
+        const RunPlace place(p, cur, a.j0, a.j1, u - a.j0, per, 128);
+        dest = row_ok ? place.index(p, tok, hd, r) : -1;
+        if (row_ok) place.describe(p, cur, tok, hd, r);
+      }
+      next(a);
       float m_ref = -INFINITY, l = 0.f;
       for (int j = a.lo; j < a.hi; ++j, ++it) {
         const uint32_t b = it & 1u, ph = (it >> 1) & 1u;
@@ -295,9 +318,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           tc::tmem_ld_32x32(tS + lane_off + (uint32_t)(c * 32), reinterpret_cast<uint32_t(&)[32]>(sv[c * 32]));
         tc::tmem_ld_wait();
         // keys of this block that the row sees
-        const bool pre = j < a.prefix_blocks;
-        const int kv0 = (pre ? j : j - a.prefix_blocks) * BN;
-        const int vis = (pre ? p.prefix_len : SEQ ? min(sees, oend) : 0) - kv0;
+        const bool pre = j < prefix_blocks;
+        const int kv0 = (pre ? j : j - prefix_blocks) * BN;
+        const int vis = (pre ? p.prefix_len : SEQ ? min(sees, a.own_end) : 0) - kv0;
         if (__any_sync(0xffffffffu, vis < BN)) {
 #pragma unroll
           for (int e = 0; e < BN; ++e)
@@ -370,7 +393,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       if (a.lo >= a.hi) {                           // no key for this tile: nothing went through the pipeline
         if (row_ok) {
           float zero[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int d = 0; d < HD; d += 4) store_row<4>(p, part, tok0 + idx, h * p.G + rg, d, zero, -INFINITY, 0.f);
+          for (int d = 0; d < HD; d += 4) store_row<4>(p, dest, tok, hd, d, zero, -INFINITY, 0.f);
         }
         continue;
       }
@@ -378,9 +401,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       tc::tc_fence_after();
       ++t;
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      __half *orow = p.out + (int64_t)(tok0 + idx) * p.so_t + (int64_t)(h * p.G + rg) * p.so_h;
-      const int64_t prow = (int64_t)part * p.T * p.Hq + row;
-      if (p.part_o && row_ok) p.part_ml[prow] = make_float2(m_ref, l);
+      __half *orow = p.out + (int64_t)tok * p.so_t + (int64_t)hd * p.so_h;
+      if (dest >= 0 && row_ok) p.part_ml[dest] = make_float2(m_ref, l);
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t o[32];
@@ -392,9 +414,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           if (lane == 0) tc::mbar_arrive(o_empty);
         }
         if (!row_ok) continue;
-        if (p.part_o) {
+        if (dest >= 0) {
           if (l != 0.f) {
-            float4 *dst = reinterpret_cast<float4 *>(p.part_o + prow * HD + c * 32);
+            float4 *dst = reinterpret_cast<float4 *>(p.part_o + dest * HD + c * 32);
 #pragma unroll
             for (int g = 0; g < 8; ++g)
               dst[g] = make_float4(__uint_as_float(o[g * 4]), __uint_as_float(o[g * 4 + 1]), __uint_as_float(o[g * 4 + 2]),
@@ -447,8 +469,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       const int share = 128 / cl, tid = threadIdx.x - 64;
       for (int i = tid; i < share * (HD / 4); i += 128) {
         const int rr = rank * share + i / (HD / 4), d = (i % (HD / 4)) * 4;
-        const int idx = (int)blockIdx.x * TB + rr / p.G;
-        if (rr >= rows_tile || idx >= ntok) continue;
+        const int idx = (int)blockIdx.x * TB + rr / p.G, hd = (int)blockIdx.z * p.G + rr % p.G;
+        if (rr >= rows_tile || idx >= cur.ntok) continue;
         float m = -INFINITY, ll = 0.f, f[4] = {0.f, 0.f, 0.f, 0.f};
         const uint32_t mrow = tc::smem_u32(&ml[rr]);
         const uint32_t orow = so + (uint32_t)(rr * HD * 4) + (((uint32_t)(d / 4) ^ (uint32_t)(rr & (HD / 4 - 1))) * 16);
@@ -463,7 +485,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           const float4 q = ld_cluster_f4(tc::map_to_rank(orow, (uint32_t)k));
           f[0] += q.x; f[1] += q.y; f[2] += q.z; f[3] += q.w;
         }
-        store_row<4>(p, part / cl, idx, h * p.G + rr % p.G, d, f, m, ll);
+        const int64_t dest = p.part_o ? (int64_t)(part / cl) * p.T * p.Hq + (int64_t)idx * p.Hq + hd : -1;
+        store_row<4>(p, dest, idx, hd, d, f, m, ll);
       }
       tc::cluster_sync_all();                                                 // no CTA leaves while its memory is read
     }
