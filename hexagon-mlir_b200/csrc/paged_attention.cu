@@ -70,7 +70,8 @@ struct RowCfg {
   // Exchange between the key groups: m, l, and 16 rows of DP / 4 columns a warp.  Heads of more than 128 leave no room
   // for it beside three stages: their tiles have 64 rows, a warp owns all keys of its 16.
   static constexpr int XCH = STAGES * 2 * KV;
-  static constexpr int OFFS = XCH + (DP > 128 ? 0 : (128 + 64 * (DP / 4 + 2)) * 4);   // cp.async: row offsets, K and V, two buffers
+  static constexpr int XLD = DP == 64 ? 18 : DP / 4 + 8;   // row pitch (40: no bank conflicts; 24 would cost the fourth CTA of 64-wide heads)
+  static constexpr int OFFS = XCH + (DP > 128 ? 0 : (128 + 64 * XLD) * 4);   // cp.async: row offsets, K and V, two buffers
   static constexpr int BARS = OFFS;                      // TMA: full and empty barrier of every stage, abort flag
   static constexpr int SMEM = OFFS + 2 * 2 * BN * 8;
   static constexpr int SMEM_TMA = BARS + 2 * STAGES * 8 + 16 + 1024;
@@ -223,7 +224,7 @@ struct Run {
       // [w, w + 1) * DP / KW from the others, one of them a round (joining 16 columns of all groups at a time, between two
       // barriers each, took 6.7 us a run; this takes a third).
       constexpr int QC = DP / KW, PC = DP / 4;                 // columns a group keeps; of them a round
-      constexpr int PN = PC / 8, LD = PC + 2;                  // 8-column tiles, row pitch
+      constexpr int PN = PC / 8, LD = RowCfg<DP>::XLD;         // 8-column tiles, row pitch
       float *sm = xch, *sl = xch + 64;                         // [KW][ROWS] each
       float *so = xch + 128 + (kw * RW + rw) * 16 * LD;        // what this warp sends: its 16 rows
       const int r0 = rw * 16 + (lane >> 2);
@@ -548,7 +549,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const Params p) {
   constexpr int SUBS = 32 / LPR;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int t = (int)(row / p.Hq), hd = (int)(row - (int64_t)t * p.Hq);
-  if (t >= tokens_used(p)) return;
+  if (t >= p.T) return;
+  const int used = tokens_used(p);
   const int64_t n = (int64_t)p.T * p.Hq;
   // The parts of a row: those of the prefix, then those of its own keys; each side either in row order, or the runs of
   // its tile where their CTAs left them.
@@ -561,7 +563,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const Params p) {
   };
   int pc = 0, pr = 0, oc = 0, orow = 0;
   int np = side(p.prefix_desc, p.prefix_desc ? 0 : p.prefix_parts, pc, pr), no = side(p.own_desc, 0, oc, orow);
-  if (np < 0 || no < 0) return;  // stored by its one run
+  if (t >= used || np < 0 || no < 0) return;  // no sequence's; stored by its one run
   const bool pcut = p.prefix_desc && np > 0, ocut = no > 0;
   if (p.prefix_desc && np == 0) np = 1;
   if (p.own_desc && no == 0) no = 1;
@@ -662,6 +664,8 @@ static Plan make_plan(const hexb_paged_attention_desc *d, int sm_count) {
   if (d->prefix_len > 0 && tc_ok && d->T * G >= 64) {
     pl.tc_prefix = true;
     const int64_t tiles = (int64_t)ceil_div(d->T, pl.tile_tokens) * d->Hkv;
+    // Two CTAs an SM.  (One, so that the stream's CTAs run beside it, takes longer: a single CTA does not keep the tensor
+    // pipe busy.  64 sequences behind 8192 keys 74 us against 65, 128 behind 16385 keys 150 against 118.)
     const int64_t ranges = clamp64(2 * sm_count / tiles, 1, clamp64((pblocks + 1) / 2, 1, 64));
     for (pl.cluster = 8; pl.cluster > ranges;) pl.cluster /= 2;
     pl.prefix_parts = (int)(ranges / pl.cluster);
