@@ -6,26 +6,35 @@
 //   min-p   of those, the ones with w_i >= min_p
 //   token   the first kept index, in index order, whose inclusive sum of w exceeds u times the kept sum
 //
-// Ties are ordered by index everywhere (the lower one first).  Drawing in index order needs no sort: each filter
-// is a cut (key, index) in the descending order, found by histograms.  NaN and -inf are never chosen; a row
-// with nothing else gives -1.
+// Ties are ordered by index everywhere (the lower one first), so each filter keeps a prefix of one descending order, and
+// a cut in it -- (key, index) -- says all.  NaN and -inf are never chosen; a row with nothing else gives -1.
 //
-// A token is a whole number, so borders decide: weights are formed in 64 bits, and sums are 64-bit sums or exact
-// integers (44 bits of the mass; two 32-bit shared-memory atomics a logit), so the result does not
-// depend on the order of the atomics.
+// A token is a whole number, so borders decide: weights and sums are formed in 64 bits, or as exact integers (44 bits of
+// the mass), and in an order that does not depend on how the threads run.
 //
-// One cluster of C CTAs owns a row: each CTA reads its slice once into shared memory and all passes run there;
-// the CTAs exchange maxima, sums and histograms through distributed shared memory.  A slice that does not fit
-// is read again from L2 by each pass.
+// Drawing in index order needs no sorted row.  A histogram of the row's values (one shared-memory atomic a logit) gives
+// the cut of top-k to a bin, and with the bins' weights a guess of the cut of top-p to a few.  Then one pass
+//   - collects the logits at or above the cut, if they are few: the rest happens in that sorted list; else
+//   - collects the cut's bins alone and sums, exactly, the mass above them and in all, which settles the cut and proves or
+//     disproves the guess; a last pass draws among what is kept.
+// Where the list would not hold the bins (thousands of equal logits) or the guess was wrong, the cut is found by
+// histograms of the keys, level by level.
+//
+// Few rows: a cluster of CTAs owns a row, each with its slice in shared memory, and exchanges maxima, sums and
+// histograms through distributed shared memory; a step costs latency only.  Many rows: one CTA a row, two an SM, the
+// passes read the row from L2; instruction issue is the bound (256 rows of 128000 fp16: 65 MB, 10 us of memory).
 #include "tc_sm100.cuh"
 
 namespace hexb {
 namespace sampling {
 
+typedef unsigned long long u64;
+
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int NB = 2048;           // histogram bins
+constexpr int CAP = 4096;          // list entries
 constexpr int MAXC = 8;
-constexpr int VEC = 4;             // elements a lane takes at a time
+constexpr int kLevels = 16;        // of the exponential's table
 
 struct Params {
   const void *x;
@@ -47,26 +56,11 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
-
-// 2^y for y <= 0 in 64 bits: y = n + f, |f| <= 1/2, Taylor series of e^(f ln 2) (degree 11: the first term left
-// out is below 0.3466^12 / 12! = 7e-15), exponent added as an integer.  Below 2^-1000: 0.
-__device__ __forceinline__ double exp2_neg(double y) {
-  if (!(y > -1000.0)) return 0.0;
-  const double n = rint(y);
-  const double f = (y - n) * 0.693147180559945309417;
-  double r = 1.0 / 39916800.0;
-  r = fma(r, f, 1.0 / 3628800.0);
-  r = fma(r, f, 1.0 / 362880.0);
-  r = fma(r, f, 1.0 / 40320.0);
-  r = fma(r, f, 1.0 / 5040.0);
-  r = fma(r, f, 1.0 / 720.0);
-  r = fma(r, f, 1.0 / 120.0);
-  r = fma(r, f, 1.0 / 24.0);
-  r = fma(r, f, 1.0 / 6.0);
-  r = fma(r, f, 0.5);
-  r = fma(r, f, 1.0);
-  r = fma(r, f, 1.0);
-  return __longlong_as_double(__double_as_longlong(r) + ((long long)n << 52));
+// A finite float in 64 bits by integer operations (the conversion instruction runs at an eighth of the rate); zero and
+// subnormal numbers come out below 2^-126, which changes no sum here.
+__device__ __forceinline__ double widen(float x) {
+  const uint32_t b = __float_as_uint(x), mag = b & 0x7fffffffu;
+  return __hiloint2double((int)((b & 0x80000000u) | ((mag >> 3) + 0x38000000u)), (int)(mag << 29));
 }
 
 // What is kept so far: keys above `key`, and of those equal to it the indices up to `index`.
@@ -76,19 +70,25 @@ struct Cut {
 };
 
 struct Shared {
-  uint32_t count[NB], hi[NB], lo[NB];
+  uint32_t count[NB];
+  u64 list[CAP];               // (key, ~index); the key histograms' two mass words lie here too
+  double mass[CAP];                 // of the sorted list: weights, then running sums
+  double table[kLevels];            // 2^(-i / kLevels)
   double warp_sum[WARPS];
-  double part[2][MAXC];             // this CTA's column of each exchange is [..][rank] of every CTA
-  float fmax[MAXC], fmin[MAXC];
-  int imin[MAXC];
-  int found_index;
-  unsigned long long scan[WARPS];
-  int bin;
-  unsigned long long before;
-  uint32_t bin_count;
-  int winner;
+  double part[2][MAXC];
   double rel;
+  u64 best[MAXC];              // (key, ~index) of the largest logit of every CTA
+  float fmin[MAXC];
+  u64 scan[WARPS];
+  float fscan[WARPS];
+  unsigned long long before;
+  uint32_t bin_count, n;            // list length
+  int found_index, bin, winner, b_k, b_p, b_last, n_last, n_first, n_guess, guessed;
+  uint32_t before_k;
+  Cut cut;
+  int cut_ok;
 };
+static_assert(2 * NB * 4 <= CAP * 8, "mass words fit the list");
 
 __device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
@@ -96,10 +96,18 @@ __device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
-__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ void st_cluster_u64(uint32_t addr, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ uint4 ld_cluster_u128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
+}
+__device__ __forceinline__ uint32_t add_cluster_u32(uint32_t addr, uint32_t v) {
+  uint32_t old;
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v) : "memory");
+  return old;
 }
 
 template <typename T, int C>
@@ -108,10 +116,12 @@ struct Row {
   Shared &s;
   const T *data;          // the slice: shared memory, or global
   int n, rank, warp, lane;
-  int w0, w1;             // this warp's contiguous part of the slice
+  int shift;              // elements between the 16-byte boundary below `data` and data
+  int v0, v1;             // this warp's contiguous part of the slice, in 16-byte vectors from that boundary
   int first;              // row index of slice element 0
-  float m;
-  double inv_t;           // log2(e) / T
+  float m, f_bin;         // maximum; bins per unit of value
+  double scale, offset;   // (x, T) -> kLevels * log2 of the weight
+  float scale32;
   int flip;
 
   __device__ Row(const Params &p_, Shared &s_) : p(p_), s(s_), flip(0) {}
@@ -124,22 +134,56 @@ struct Row {
     const uint32_t l = tc::smem_u32(a);
     return C > 1 ? tc::map_to_rank(l, (uint32_t)r) : l;
   }
-  __device__ __forceinline__ float at(int i) const {
-    const float v = to_f32<T>(data[i]);
-    return v != v ? -INFINITY : v;
-  }
+  // 2^(y / kLevels) for y = kLevels * log2(e) * (v - m) / T <= 0, in 64 bits: y = k + f, |f| <= 1/2; 2^(k / kLevels) from the table
+  // and the exponent, 2^(f / kLevels) by its Taylor series (degree 5: the next term is below 0.0217^6 / 720 = 2e-13).
   __device__ __forceinline__ double weight(float v) const {
-    return v == m ? 1.0 : exp2_neg(((double)v - (double)m) * inv_t);
+    if (v == m) return 1.0;
+    const double y = fma(widen(v), scale, offset);
+    if (!(y > -16000.0)) return 0.0;                 // 2^-1000
+    const double magic = 6755399441055744.0;         // 1.5 * 2^52: the sum's low word is the rounded y
+    const double z = y + magic;
+    const int k = __double2loint(z);
+    const double f = y - (z - magic);
+    constexpr double L = 0.693147180559945309417 / kLevels;
+    double r = L * L * L * L * L / 120.0;
+    r = fma(r, f, L * L * L * L / 24.0);
+    r = fma(r, f, L * L * L / 6.0);
+    r = fma(r, f, L * L / 2.0);
+    r = fma(r, f, L);
+    r = fma(r, f, 1.0);
+    const double w = r * s.table[-k & (kLevels - 1)];
+    return __hiloint2double(__double2hiint(w) - ((-k) / kLevels << 20), __double2loint(w));
   }
   __device__ __forceinline__ bool kept(const Cut &c, float v, int i) const {
     const uint32_t k = key_of(v);
     return v > -INFINITY && (k > c.key || (k == c.key && i <= c.index));
   }
-  // f(value, row index) for every element of this warp's part
+  __device__ __forceinline__ int bin_of(float v) const {
+    const float d = v == m ? 0.0f : m - v;
+    return (int)fminf(d * f_bin, (float)(NB - 1));
+  }
+  // f(value, row index) for the elements of vector v (NaN arrives as -inf)
   template <typename F>
-  __device__ __forceinline__ void each(F &&f) {
-#pragma unroll 4
-    for (int i = w0 + lane; i < w1; i += 32) f(at(i), first + i);
+  __device__ __forceinline__ void vector(int v, F &&f) const {
+    constexpr int E = Vec16<T>::N;
+    const int i = v * E - shift;
+    float x[E];
+    if (i >= 0 && i + E <= n) {
+      Vec16<T> q;
+      q.raw = *reinterpret_cast<const decltype(q.raw) *>(data + i);
+      q.unpack(x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = i + e >= 0 && i + e < n ? to_f32<T>(data[i + e]) : -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) f(x[e] != x[e] ? -INFINITY : x[e], first + i + e);
+  }
+  // f for every element of this warp's part, and -inf for some places beside it
+  template <typename F>
+  __device__ __forceinline__ void each(F &&f) const {
+#pragma unroll 2
+    for (int v = v0 + lane; v < v1; v += 32) vector(v, f);
   }
 
   // Sum of one 64-bit value per thread over the cluster: lanes, warps in order, CTAs in order.  Also leaves the
@@ -166,8 +210,8 @@ struct Row {
     return total;
   }
 
-  // Lowest row index at which the inclusive sum of f exceeds target(total); -1 if the sum is empty.  The CTA
-  // that holds it returns it, others return -1.
+  // Lowest row index at which the inclusive sum of f exceeds target(total); -1 if the sum is empty.  The warp that
+  // finds it returns it, all others -1.
   template <typename F, typename G>
   __device__ int ordered_find(F &&f, G &&target) {
     double v = 0.0;
@@ -204,70 +248,413 @@ struct Row {
     }
     __syncthreads();
     if (warp != s.winner) return -1;
+    // a lane's vector first, then the element in it
+    constexpr int E = Vec16<T>::N;
     double run = s.rel;
     int last = -1;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-      const int i = i0 + lane;
-      const double own = i < w1 ? f(at(i), first + i) : 0.0;
-      double incl = own;
+    for (int vb = v0; vb < v1; vb += 32) {
+      const int vv = vb + lane;
+      double own[E], sum = 0.0;
+      int at = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) own[e] = 0.0;
+      if (vv < v1) {
+        int e = 0;
+        vector(vv, [&](float x, int i) {
+          own[e++] = f(x, i);
+          sum += own[e - 1];
+        });
+        at = first + vv * E - shift;
+      }
+      double incl = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const double up = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += up;
       }
-      const unsigned any = __ballot_sync(0xffffffffu, own > 0.0);
-      if (any) last = first + i0 + 31 - __clz(any);
-      const unsigned over = __ballot_sync(0xffffffffu, own > 0.0 && run + incl > t);
-      if (over) return first + i0 + __ffs(over) - 1;
+      const unsigned any = __ballot_sync(0xffffffffu, sum > 0.0);
+      const unsigned over = __ballot_sync(0xffffffffu, sum > 0.0 && run + incl > t);
+      // the lane that crosses, or the last that holds anything: its elements in order
+      const int from = over ? __ffs(over) - 1 : any ? 31 - __clz(any) : -1;
+      int mine = -1;
+      if (lane == from) {
+        double c = run + (incl - sum);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          c += own[e];
+          if (own[e] > 0.0 && (mine < 0 || !(c - own[e] > t))) mine = at + e;
+        }
+      }
+      if (from >= 0) {
+        last = __shfl_sync(0xffffffffu, mine, from);
+        if (over) return last;
+      }
       run += __shfl_sync(0xffffffffu, incl, 31);
     }
     return last;  // the sums of the scan and of the lanes may round apart: the last one then
   }
 
-  // Histogram bin in which the running total of `value` first reaches `need` (bins in descending key order).
-  // count / hi / lo of the cluster are summed by every CTA alike.  Leaves bin, the total before it and its count.
+  __device__ void clear(bool mass) {
+    for (int i = threadIdx.x; i < NB; i += THREADS) s.count[i] = 0;
+    if (mass) {
+      uint32_t *w = reinterpret_cast<uint32_t *>(s.list);
+      for (int i = threadIdx.x; i < 2 * NB; i += THREADS) w[i] = 0;
+    }
+    __syncthreads();
+  }
+  // This thread's four bins of the cluster's histogram (0: counts, 1 and 2: the words of the mass).
+  __device__ __forceinline__ uint4 bins4(int which) {
+    const uint32_t *h = which == 0 ? s.count : reinterpret_cast<const uint32_t *>(s.list) + (which - 1) * NB;
+    uint4 c = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < C; ++r) {
+      const uint4 v = C > 1 ? ld_cluster_u128(peer(h + threadIdx.x * 4, r)) : *reinterpret_cast<const uint4 *>(h + threadIdx.x * 4);
+      c.x += v.x; c.y += v.y; c.z += v.z; c.w += v.w;
+    }
+    return c;
+  }
+  // exclusive prefix over the threads of the CTA
+  template <typename U>
+  __device__ __forceinline__ U exclusive(U v, U *scratch) {
+    U incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const U up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    __syncthreads();
+    if (lane == 31) scratch[warp] = incl;
+    __syncthreads();
+    U e = incl - v;
+    for (int w = 0; w < warp; ++w) e += scratch[w];
+    return e;
+  }
+
+  // ------------------------------------------------------------ the plan: histogram of values
+  // Counts over at most 32 below the maximum, linear in the value (logits spread evenly there, so the atomics do).
+  // Leaves: b_k, before_k  bin of the k-th logit and the count before it
+  //         b_p            guess of the bin where p of the mass (of what top-k leaves) is reached
+  //         b_last         the last bin that the list needs, n_last logits up to it; guessed: b_p set it
+  //         n_first, n_guess   logits before bin b_p - 3, and up to bin b_p + 3
+  __device__ void plan(const Cut &in, int top_k, float top_p, float min_p, float lowest) {
+    const float range = fminf(m - lowest, 32.0f);
+    f_bin = range > 1e-20f ? (float)NB / range : 0.0f;
+    clear(false);
+    each([&](float v, int) {
+      if (v > -INFINITY) atomicAdd(&s.count[bin_of(v)], 1u);
+    });
+    if (threadIdx.x == 0) {
+      s.b_k = s.b_p = NB - 1;
+      s.before_k = 0;
+      s.n_last = s.n_first = s.n_guess = 0;
+    }
+    cluster_barrier();
+    const uint4 c4 = bins4(0);
+    const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
+    const u64 before = exclusive<u64>((u64)c[0] + c[1] + c[2] + c[3], s.scan);
+    const int b0 = threadIdx.x * 4;
+    if (top_k > 0) {
+      u64 e = before;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (e < (u64)top_k && e + c[i] >= (u64)top_k) {
+          s.b_k = b0 + i;
+          s.before_k = (uint32_t)e;
+        }
+        e += c[i];
+      }
+    }
+    __syncthreads();
+    const int b_k = s.b_k;
+    if (top_p < 1.0f) {
+      float w[4], sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float centre = f_bin > 0.f ? ((float)(b0 + i) + 0.5f) / f_bin : 0.f;
+        w[i] = b0 + i <= b_k ? (float)c[i] * exp2f(-centre * scale32) : 0.f;
+        sum += w[i];
+      }
+      float e = exclusive<float>(sum, s.fscan);
+      float all = 0.f;
+      for (int i = 0; i < WARPS; ++i) all += s.fscan[i];
+      const float need = fmaxf(top_p * all, 1e-30f);
+      bool hit = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!hit && c[i] && e < need && e + w[i] >= need) {
+          atomicMin(&s.b_p, b0 + i);
+          hit = true;
+        }
+        e += w[i];
+      }
+    }
+    __syncthreads();
+    int limit = b_k;                              // of what any filter but top-p keeps
+    if (min_p > 0.0f) {
+      const float d = -log2f(min_p) / scale32;    // the first difference that min_p drops, to 32 bits
+      limit = min(limit, (int)fminf(d * f_bin, (float)(NB - 4)) + 2);
+    }
+    // the mass that top-p takes its share of is top-k's, if there is one: then the list has to hold that
+    const int last = top_p < 1.0f ? (top_k > 0 ? b_k : min(limit, s.b_p + 3)) : limit;
+    u64 e = before;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (b0 + i == s.b_p - 3) s.n_first = (int)e;
+      e += c[i];
+      if (b0 + i == last) s.n_last = (int)e;
+      if (b0 + i == min(s.b_p + 3, NB - 1)) s.n_guess = (int)e;
+    }
+    if (threadIdx.x == 0) {
+      s.b_last = last;
+      s.guessed = last < limit;
+    }
+    cluster_barrier();  // every CTA has read the histograms
+  }
+
+  // ------------------------------------------------------------ the list
+  __device__ __forceinline__ void list_reset() {
+    if (threadIdx.x == 0) s.n = 0;
+    cluster_barrier();
+  }
+  // Appends (v, i) to the list of CTA 0 where `take`; the whole warp calls it.
+  __device__ __forceinline__ void append(bool take, float v, int i) {
+    const unsigned who = __ballot_sync(0xffffffffu, take);
+    if (!who) return;
+    uint32_t at = 0;
+    if (lane == __ffs(who) - 1) at = C > 1 ? add_cluster_u32(peer(&s.n, 0), __popc(who)) : atomicAdd(&s.n, (uint32_t)__popc(who));
+    at = __shfl_sync(0xffffffffu, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1u));
+    if (take && at < CAP) {
+      const u64 entry = (u64)key_of(v) << 32 | (uint32_t)~i;
+      if (C > 1) st_cluster_u64(peer(&s.list[at], 0), entry);
+      else s.list[at] = entry;
+    }
+  }
+  // f(take, value, index) by whole warps
+  template <typename F>
+  __device__ __forceinline__ void each_warp(F &&f) {
+    constexpr int E = Vec16<T>::N;
+    for (int vb = v0; vb < v1; vb += 32) {
+      const int vv = vb + lane;
+      float x[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = -INFINITY;
+      int at = 0;
+      if (vv < v1) {
+        int e = 0;
+        vector(vv, [&](float v, int) { x[e++] = v; });
+        at = first + vv * E - shift;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) f(x[e], at + e);
+    }
+  }
+  // Descending bitonic sort of the list (all threads of CTA 0).
+  __device__ void sort(u64 *a, int n) {
+    int size = 2;
+    while (size < n) size *= 2;
+    for (int i = n + threadIdx.x; i < size; i += THREADS) a[i] = 0;
+    __syncthreads();
+    for (int k = 2; k <= size; k *= 2)
+      for (int j = k / 2; j > 0; j /= 2) {
+        for (int i = threadIdx.x; i < size / 2; i += THREADS) {
+          const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+          const u64 x = a[lo], y = a[hi];
+          if ((x < y) == ((lo & k) == 0)) {
+            a[lo] = y;
+            a[hi] = x;
+          }
+        }
+        __syncthreads();
+      }
+  }
+  // s.mass[i] <- sum of the weights of list entries 0 .. i (CTA 0).  Fixed order: eight consecutive entries a thread.
+  __device__ void accumulate(int n) {
+    constexpr int PER = CAP / THREADS;
+    double w[PER], sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = threadIdx.x * PER + i;
+      w[i] = e < n ? weight(value_of((uint32_t)(s.list[e] >> 32))) : 0.0;
+      sum += w[i];
+    }
+    double run = exclusive<double>(sum, s.warp_sum);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      run += w[i];
+      s.mass[threadIdx.x * PER + i] = run;
+    }
+    __syncthreads();
+  }
+  // First i < n with ok(i) false (ok holds for a prefix); all threads of CTA 0.
+  template <typename F>
+  __device__ int prefix_length(int n, F &&ok) {
+    __syncthreads();
+    if (threadIdx.x == 0) s.found_index = 0;
+    __syncthreads();
+    int mine = 0;
+    for (int i = threadIdx.x; i < n; i += THREADS)
+      if (ok(i)) mine = i + 1;
+    if (mine) atomicMax(&s.found_index, mine);
+    __syncthreads();
+    return s.found_index;
+  }
+  // The cut that CTA 0 found, to all.
+  __device__ bool broadcast(Cut &c) {
+    if (C > 1) {
+      if (rank == 0 && threadIdx.x < C) {
+        st_cluster_u32(peer(&s.cut.key, threadIdx.x), s.cut.key);
+        st_cluster_u32(peer(&s.cut.index, threadIdx.x), (uint32_t)s.cut.index);
+        st_cluster_u32(peer(&s.cut_ok, threadIdx.x), (uint32_t)s.cut_ok);
+      }
+    }
+    cluster_barrier();
+    const bool ok = s.cut_ok != 0;
+    if (ok) c = s.cut;
+    cluster_barrier();
+    return ok;
+  }
+
+  // ------------------------------------------------------------ everything that is needed fits the list
+  // CTA 0 returns the token (thread 0), others -1; -2 in every thread: the guess of top-p was too short.
+  __device__ int from_list(int top_k, float top_p, float min_p, float u) {
+    const int last = s.b_last;
+    list_reset();
+    double sum = 0.0, cta[C];
+    const bool total_needed = top_p < 1.0f && top_k <= 0;
+    each_warp([&](float v, int i) {
+      append(v > -INFINITY && bin_of(v) <= last, v, i);
+      if (total_needed && v > -INFINITY) sum += weight(v);
+    });
+    double total = 0.0;
+    if (total_needed) total = cluster_total(sum, cta);
+    cluster_barrier();
+    int token = -1;
+    bool short_list = false;
+    if (rank == 0) {
+      const int n = (int)min(s.n, (uint32_t)CAP);
+      sort(s.list, n);
+      accumulate(n);
+      int keep = top_k > 0 ? min(top_k, n) : n;
+      if (top_p < 1.0f) {
+        if (!total_needed) total = s.mass[keep - 1];
+        const double need = (double)top_p * total;
+        const int fits = prefix_length(keep, [&](int i) { return i == 0 || s.mass[i - 1] < need; });
+        // every entry belongs to the nucleus and the guess ended the list: the next logit, which is not here, may too
+        short_list = s.guessed && fits == n && s.mass[n - 1] < need;
+        keep = fits;
+      }
+      if (min_p > 0.0f) {
+        const double w_min = (double)min_p;
+        keep = prefix_length(keep, [&](int i) { return weight(value_of((uint32_t)(s.list[i] >> 32))) >= w_min; });
+        short_list = short_list && keep == n;
+      }
+      if (!short_list) {
+        if (keep <= 1) {
+          token = (int)~(uint32_t)s.list[0];
+        } else {
+          // the kept entries by index: (~index, key) descending
+          for (int i = threadIdx.x; i < keep; i += THREADS) s.list[i] = s.list[i] << 32 | s.list[i] >> 32;
+          __syncthreads();
+          sort(s.list, keep);
+          for (int i = threadIdx.x; i < keep; i += THREADS) s.list[i] = s.list[i] << 32 | s.list[i] >> 32;
+          __syncthreads();
+          accumulate(keep);
+          const double t = (double)u * s.mass[keep - 1];
+          const int at = prefix_length(keep, [&](int i) { return s.mass[i] <= t; });
+          token = (int)~(uint32_t)s.list[min(at, keep - 1)];
+        }
+        if (threadIdx.x) token = -1;
+      }
+      if (threadIdx.x == 0) s.cut_ok = short_list;
+      __syncthreads();
+    }
+    Cut unused;
+    return broadcast(unused) ? -2 : token;
+  }
+
+  // ------------------------------------------------------------ a cut whose bins fit the list
+  // k-th logit: it is in bin b_k.
+  __device__ bool refine_k(Cut &cut, int top_k) {
+    const int b = s.b_k;
+    const int rank_in = top_k - (int)s.before_k;     // 1 ..
+    list_reset();
+    each_warp([&](float v, int i) { append(v > -INFINITY && bin_of(v) == b, v, i); });
+    cluster_barrier();
+    if (rank == 0) {
+      const int n = (int)min(s.n, (uint32_t)CAP);
+      const bool ok = s.n <= CAP && rank_in <= n;
+      if (ok) sort(s.list, n);
+      if (threadIdx.x == 0) {
+        s.cut_ok = ok;
+        if (ok) s.cut = {(uint32_t)(s.list[rank_in - 1] >> 32), (int)~(uint32_t)s.list[rank_in - 1]};
+      }
+      __syncthreads();
+    }
+    return broadcast(cut);
+  }
+  // p of the mass: guessed to lie in bins [b_p - 3, b_p + 3].
+  __device__ bool refine_p(Cut &cut, float top_p) {
+    const int lo = s.b_p - 3, hi = s.b_p + 3;
+    list_reset();
+    double sum = 0.0, above = 0.0, cta[C];
+    each_warp([&](float v, int i) {
+      const bool k = kept(cut, v, i);
+      const int b = k ? bin_of(v) : NB;
+      append(b >= lo && b <= hi, v, i);
+      if (k) {
+        const double w = weight(v);
+        sum += w;
+        if (b < lo) above += w;
+      }
+    });
+    const double total = cluster_total(sum, cta);
+    const double over = cluster_total(above, cta);
+    cluster_barrier();
+    if (rank == 0) {
+      const int n = (int)min(s.n, (uint32_t)CAP);
+      bool ok = s.n <= CAP && n > 0;
+      if (ok) {
+        sort(s.list, n);
+        accumulate(n);
+        const double need = (double)top_p * total;
+        const int fits = prefix_length(n, [&](int i) { return over + (i ? s.mass[i - 1] : 0.0) < need; });
+        ok = (fits > 0 || lo <= 0) && (fits < n || over + s.mass[n - 1] >= need || hi >= NB - 1);
+        const int at = max(fits, 1) - 1;
+        if (threadIdx.x == 0) s.cut = {(uint32_t)(s.list[at] >> 32), (int)~(uint32_t)s.list[at]};
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) s.cut_ok = ok;
+      __syncthreads();
+    }
+    return broadcast(cut);
+  }
+
+  // ------------------------------------------------------------ a cut by histograms alone
+  // Bin in which the running total first reaches `need` (bins in descending key order).
   template <bool MASS>
   __device__ void find_bin(double need) {
     cluster_barrier();  // all histograms are complete
-    constexpr int PER = NB / THREADS;
-    unsigned long long v[PER];
-    uint32_t cnt[PER];
-    unsigned long long sum = 0;
+    const uint4 c4 = bins4(0), h4 = MASS ? bins4(1) : make_uint4(0, 0, 0, 0), l4 = MASS ? bins4(2) : make_uint4(0, 0, 0, 0);
+    const uint32_t cnt[4] = {c4.x, c4.y, c4.z, c4.w}, h[4] = {h4.x, h4.y, h4.z, h4.w}, l[4] = {l4.x, l4.y, l4.z, l4.w};
+    u64 v[4], sum = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int b = threadIdx.x * PER + i;
-      cnt[i] = 0;
-      v[i] = 0;
-#pragma unroll
-      for (int r = 0; r < C; ++r) {
-        cnt[i] += ld_cluster_u32(peer(&s.count[b], r));
-        if (MASS) v[i] += ((unsigned long long)ld_cluster_u32(peer(&s.hi[b], r)) << 14) + ld_cluster_u32(peer(&s.lo[b], r));
-      }
-      if (!MASS) v[i] = cnt[i];
+    for (int i = 0; i < 4; ++i) {
+      v[i] = MASS ? ((u64)h[i] << 14) + l[i] : cnt[i];
       sum += v[i];
     }
-    unsigned long long incl = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    if (lane == 31) s.scan[warp] = incl;
     if (threadIdx.x == 0) s.bin = -1;
-    __syncthreads();
-    unsigned long long excl = incl - sum;
-    for (int w = 0; w < warp; ++w) excl += s.scan[w];
+    const u64 excl = exclusive<u64>(sum, s.scan);
     // the crossing bin; without one (rounding at the far end) the last bin that holds anything
     int last = -1;
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (cnt[i]) last = threadIdx.x * PER + i;
-    unsigned long long e = excl;
+    for (int i = 0; i < 4; ++i)
+      if (cnt[i]) last = threadIdx.x * 4 + i;
+    u64 e = excl;
     bool hit = false;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
+    for (int i = 0; i < 4; ++i) {
       if (cnt[i] && (double)e < need && (double)(e + v[i]) >= need) {
-        s.bin = threadIdx.x * PER + i;
+        s.bin = threadIdx.x * 4 + i;
         s.before = e;
         s.bin_count = cnt[i];
         hit = true;
@@ -279,15 +666,15 @@ struct Row {
       atomicMax(&s.bin, last);
       __syncthreads();
       const int b = s.bin;
-      if (b / PER == (int)threadIdx.x) {
-        unsigned long long f = excl;
+      if (b / 4 == (int)threadIdx.x) {
+        u64 g = excl;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          if (threadIdx.x * PER + i == b) {
-            s.before = f;
+        for (int i = 0; i < 4; ++i) {
+          if (threadIdx.x * 4 + i == b) {
+            s.before = g;
             s.bin_count = cnt[i];
           }
-          f += v[i];
+          g += v[i];
         }
       }
       __syncthreads();
@@ -295,76 +682,41 @@ struct Row {
     cluster_barrier();  // every CTA has read the histograms
   }
 
-  __device__ void clear() {
-    for (int i = threadIdx.x; i < NB; i += THREADS) s.count[i] = s.hi[i] = s.lo[i] = 0;
-    __syncthreads();
-  }
-
-  // The cut of top-k (MASS false: `need` elements) or top-p (MASS true: `need` units of mass; unit = 1 / scale):
-  // first by value, linear over at most 64 below the maximum -- logits spread evenly there, so the atomics do --
-  // then by key within the bin until a bin is one key.
+  // The cut of top-k (MASS false: `need` elements) or top-p (MASS true: `need` units of mass; unit = 1 / units): bins of
+  // keys, narrowed until a bin is one key.
   template <bool MASS>
-  __device__ Cut descend(const Cut &in, double need, double scale, float lowest) {
-    const float range = fminf(m - lowest, 64.0f);
-    const float f = range > 1e-20f ? (float)NB / range : 0.0f;
-    auto bin_of = [&](float v) {
-      const float d = v == m ? 0.0f : m - v;
-      return (int)fminf(d * f, (float)(NB - 1));
-    };
-    auto add = [&](int b, float v) {
-      atomicAdd(&s.count[b], 1u);
-      if (MASS) {
-        const unsigned long long q = __double2ull_rn(weight(v) * scale);
-        atomicAdd(&s.hi[b], (uint32_t)(q >> 14));
-        atomicAdd(&s.lo[b], (uint32_t)(q & 16383u));
-      }
-    };
-    clear();
-    each([&](float v, int i) {
-      if (kept(in, v, i)) add(bin_of(v), v);
-    });
-    find_bin<MASS>(need);
-    unsigned long long before = s.before;
-    const int b = s.bin;
-    // keys of the bin: bin_of does not rise with the key
-    uint32_t lo = key_of(lowest), hi = key_of(m);
-    {
-      uint32_t l = lo, h = hi;      // lowest key with bin <= b
-      while (l < h) {
-        const uint32_t mid = l + (h - l) / 2;
-        if (bin_of(value_of(mid)) <= b) h = mid;
-        else l = mid + 1;
-      }
-      const uint32_t first_key = l;
-      l = first_key, h = hi;        // highest key with bin >= b
-      while (l < h) {
-        const uint32_t mid = l + (h - l + 1) / 2;
-        if (bin_of(value_of(mid)) >= b) l = mid;
-        else h = mid - 1;
-      }
-      lo = first_key;
-      hi = l;
-    }
+  __device__ Cut descend(const Cut &in, double need, double units, float lowest) {
     constexpr int KS = sizeof(T) == 2 ? 13 : 0;  // a widened fp16 value leaves the low 13 bits of its key alone
+    uint32_t *hi_words = reinterpret_cast<uint32_t *>(s.list), *lo_words = hi_words + NB;
+    uint32_t lo = key_of(lowest), hi = key_of(m);
+    u64 before = 0;
     while (true) {
       const uint32_t span = (hi >> KS) - (lo >> KS);   // keys - 1
       int sh = 0;
       while ((span >> sh) >= (uint32_t)NB) ++sh;
       __syncthreads();
-      clear();
+      clear(MASS);
       each([&](float v, int i) {
         const uint32_t k = key_of(v);
-        if (k >= lo && k <= hi && kept(in, v, i)) add((int)(((hi >> KS) - (k >> KS)) >> sh), v);
+        if (k >= lo && k <= hi && kept(in, v, i)) {
+          const uint32_t b = ((hi >> KS) - (k >> KS)) >> sh;
+          atomicAdd(&s.count[b], 1u);
+          if (MASS) {
+            const u64 q = __double2ull_rn(weight(v) * units);
+            atomicAdd(&hi_words[b], (uint32_t)(q >> 14));
+            atomicAdd(&lo_words[b], (uint32_t)(q & 16383u));
+          }
+        }
       });
       find_bin<MASS>(need - (double)before);
-      const uint32_t bb = (uint32_t)s.bin;
+      const uint32_t b = (uint32_t)s.bin;
       before += s.before;
-      const uint32_t top = (hi >> KS) - (bb << sh);
+      const uint32_t top = (hi >> KS) - (b << sh);
       if (sh == 0) {
         const uint32_t k = KS ? (top << KS | (top & (0x80000000u >> KS) ? 0u : (1u << KS) - 1u)) : top;
         const uint32_t ties = s.bin_count;
         double t;
-        if (MASS) t = ceil((need - (double)before) / (weight(value_of(k)) * scale));
+        if (MASS) t = ceil((need - (double)before) / (weight(value_of(k)) * units));
         else t = need - (double)before;
         if (!(t > 1.0)) t = 1.0;
         Cut c = {k, 0x7fffffff};
@@ -381,7 +733,7 @@ struct Row {
   __device__ int tie_index(const Cut &in, uint32_t k, double t) {
     const int i = ordered_find([&](float v, int j) { return key_of(v) == k && kept(in, v, j) ? 1.0 : 0.0; },
                                [&](double) { return t - 0.5; });
-    if (i >= 0 && (threadIdx.x & 31) == 0)
+    if (i >= 0 && lane == 0)
       for (int r = 0; r < C; ++r) st_cluster_u32(peer(&s.found_index, r), (uint32_t)i);
     cluster_barrier();
     const int at_index = s.found_index;
@@ -391,10 +743,11 @@ struct Row {
 };
 
 template <typename T, int C>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 2)
 sample_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t dyn[];
-  __shared__ Shared s;
+  Shared &s = *reinterpret_cast<Shared *>(dyn);
+  constexpr int E = Vec16<T>::N;
   Row<T, C> r(p, s);
   const int row = blockIdx.x / C;
   r.rank = C > 1 ? (int)tc::cluster_ctarank() : 0;
@@ -403,99 +756,132 @@ sample_kernel(const Params p) {
   r.first = r.rank * p.slice;
   r.n = max(0, min(p.slice, p.V - r.first));
   const T *src = static_cast<const T *>(p.x) + (int64_t)row * p.row_stride + r.first;
+  if (threadIdx.x < kLevels) s.table[threadIdx.x] = exp2(-(double)threadIdx.x / kLevels);
   // the peers' shared memory may be written once every CTA of the cluster has started
   if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   pdl_wait();
-  float T0 = p.temperature ? p.temperature[row] : p.temperature0;
-  float top_p = p.top_p ? p.top_p[row] : p.top_p0;
-  float min_p = p.min_p ? p.min_p[row] : p.min_p0;
+  const float T0 = p.temperature ? p.temperature[row] : p.temperature0;
+  const float top_p = p.top_p ? p.top_p[row] : p.top_p0;
+  const float min_p = fminf(fmaxf(p.min_p ? p.min_p[row] : p.min_p0, 0.0f), 1.0f);  // the largest logit (w = 1) always stays
   int top_k = p.top_k ? p.top_k[row] : p.top_k0;
-  float u = fminf(fmaxf(p.u[row], 0.0f), 0.99999994f);
+  const float u = fminf(fmaxf(p.u[row], 0.0f), 0.99999994f);
 
-  const int per = ((p.slice + WARPS - 1) / WARPS + 31) / 32 * 32;
-  r.w0 = min(r.warp * per, r.n);
-  r.w1 = min(r.w0 + per, r.n);
-  float mx = -INFINITY, mn = INFINITY;
-  auto seen = [&](float v) {
-    if (v == v) {
-      mx = fmaxf(mx, v);
-      if (v > -INFINITY) mn = fminf(mn, v);
-    }
-  };
-  if (p.resident) {
-    T *dst = reinterpret_cast<T *>(dyn);
-    constexpr int E = 16 / sizeof(T);
-    // 16-byte loads between the first and the last aligned address of the slice, single elements around them
-    const int head = min(r.n, (int)(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)));
-    const int vecs = (r.n - head) / E;
-    dst += (E - head) % E;  // the vectors are aligned in shared memory too
-    r.data = dst;
-    for (int i = threadIdx.x; i < head; i += THREADS) seen(to_f32<T>(dst[i] = src[i]));
-    for (int i = head + vecs * E + threadIdx.x; i < r.n; i += THREADS) seen(to_f32<T>(dst[i] = src[i]));
-#pragma unroll 8
-    for (int i = threadIdx.x; i < vecs; i += THREADS) {
-      Vec16<T> v;
-      v.raw = ld_stream_as<decltype(v.raw)>(src + head + i * E);
-      *reinterpret_cast<decltype(v.raw) *>(dst + head + i * E) = v.raw;
-      float f[E];
-      v.unpack(f);
+  r.shift = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
+  const int vecs = (r.n + r.shift + E - 1) / E, per = (vecs + WARPS - 1) / WARPS;
+  r.v0 = min(r.warp * per, vecs);
+  r.v1 = min(r.v0 + per, vecs);
+  r.data = src;
+  T *copy = reinterpret_cast<T *>(dyn + (sizeof(Shared) + 15) / 16 * 16) + r.shift;  // as aligned as the source
+  u64 best = 0;
+  float mn = INFINITY;
+#pragma unroll 4
+  for (int v = r.v0 + r.lane; v < r.v1; v += 32) {
+    const int i = v * E - r.shift;
+    float x[E];
+    if (i >= 0 && i + E <= r.n) {
+      Vec16<T> q;
+      q.raw = *reinterpret_cast<const decltype(q.raw) *>(src + i);
+      if (p.resident) *reinterpret_cast<decltype(q.raw) *>(copy + i) = q.raw;
+      q.unpack(x);
+    } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) seen(f[e]);
+      for (int e = 0; e < E; ++e) {
+        x[e] = -INFINITY;
+        if (i + e >= 0 && i + e < r.n) {
+          const T one = src[i + e];
+          if (p.resident) copy[i + e] = one;
+          x[e] = to_f32<T>(one);
+        }
+      }
     }
-  } else {
-    r.data = src;
-    for (int i = threadIdx.x; i < r.n; i += THREADS) seen(to_f32<T>(src[i]));
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (x[e] > -INFINITY) {  // neither NaN nor -inf
+        top = fmaxf(top, x[e]);
+        mn = fminf(mn, x[e]);
+      }
+    }
+    if (top > -INFINITY && (best == 0 || key_of(top) > (uint32_t)(best >> 32))) {  // a lane's indices rise: the first stays
+      int at = 0;
+#pragma unroll
+      for (int e = E - 1; e >= 0; --e)
+        if (x[e] == top) at = e;
+      best = (u64)key_of(top) << 32 | (uint32_t)~(r.first + i + at);
+    }
   }
-  mx = warp_max(mx);
+  if (p.resident) r.data = copy;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   mn = -warp_max(-mn);
   if (r.lane == 0) {
-    s.scan[r.warp] = ((unsigned long long)__float_as_uint(mx) << 32) | __float_as_uint(mn);
+    s.scan[r.warp] = best;
+    s.fscan[r.warp] = mn;
   }
   __syncthreads();
   if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (threadIdx.x < C) {
     for (int w = 0; w < WARPS; ++w) {
-      mx = fmaxf(w ? mx : -INFINITY, __uint_as_float((uint32_t)(s.scan[w] >> 32)));
-      mn = fminf(w ? mn : INFINITY, __uint_as_float((uint32_t)s.scan[w]));
+      best = max(w ? best : 0ull, s.scan[w]);
+      mn = fminf(w ? mn : INFINITY, s.fscan[w]);
     }
-    st_cluster_u32(r.peer(&s.fmax[r.rank], threadIdx.x), __float_as_uint(mx));
+    st_cluster_u64(r.peer(&s.best[r.rank], threadIdx.x), best);
     st_cluster_u32(r.peer(&s.fmin[r.rank], threadIdx.x), __float_as_uint(mn));
   }
   r.cluster_barrier();
-  mx = -INFINITY;
+  best = 0;
   mn = INFINITY;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    mx = fmaxf(mx, s.fmax[c]);
+    best = max(best, s.best[c]);
     mn = fminf(mn, s.fmin[c]);
   }
-  r.m = mx;
-  int token = -1;          // held by the CTA (and warp) that found it
-  if (mx == -INFINITY) {
-    if (r.rank == 0) token = -2;  // nothing to choose from
+  int token = -1;          // held by the thread that stores it
+  const bool speaker = r.rank == 0 && threadIdx.x == 0;
+  if (best == 0) {
+    if (speaker) p.out[row] = -1;  // nothing to choose from
   } else if (!(T0 > 0.0f) || top_k == 1) {
-    token = r.ordered_find([&](float v, int) { return v == mx ? 1.0 : 0.0; }, [](double) { return 0.5; });
+    if (speaker) token = (int)~(uint32_t)best;
   } else {
-    r.inv_t = 1.4426950408889634074 / (double)T0;
+    r.m = value_of((uint32_t)(best >> 32));
+    const double c = 1.4426950408889634074 / (double)T0;
+    r.scale = c * kLevels;
+    r.offset = -(double)r.m * r.scale;
+    r.scale32 = (float)c;
+    if (top_k >= p.V) top_k = 0;
     Cut cut = {0u, 0x7fffffff};
-    if (top_k > 0 && top_k < p.V) cut = r.template descend<false>(cut, (double)top_k, 0.0, mn);
-    if (top_p < 1.0f) {
-      double part = 0.0, cta[C];
-      r.each([&](float v, int i) { if (r.kept(cut, v, i)) part += r.weight(v); });
-      const double total = r.cluster_total(part, cta);
-      const double scale = 17592186044416.0 / total;  // 2^44 units
-      cut = r.template descend<true>(cut, fmax((double)top_p * 17592186044416.0, 1.0), scale, mn);
+    bool drawn = false;
+    if (top_k > 0 || top_p < 1.0f) {
+      r.plan(cut, top_k, top_p, min_p, mn);
+      if (s.n_last <= CAP) {
+        token = r.from_list(top_k, top_p, min_p, u);
+        drawn = token != -2;
+        if (!drawn) token = -1;
+      }
+      if (!drawn) {
+        const int n_p = s.n_guess - s.n_first;   // logits around the guess
+        if (top_k > 0 && !r.refine_k(cut, top_k)) cut = r.template descend<false>(cut, (double)top_k, 0.0, mn);
+        if (top_p < 1.0f && !(n_p <= CAP && r.refine_p(cut, top_p))) {
+          double part = 0.0, cta[C];
+          r.each([&](float v, int i) { if (r.kept(cut, v, i)) part += r.weight(v); });
+          const double units = 17592186044416.0 / r.cluster_total(part, cta);  // 2^44 in all
+          cut = r.template descend<true>(cut, fmax((double)top_p * 17592186044416.0, 1.0), units, mn);
+        }
+      }
     }
-    const double floor_w = (double)fminf(fmaxf(min_p, 0.0f), 1.0f);  // the largest logit (w = 1) always stays
-    token = r.ordered_find(
-        [&](float v, int i) {
-          if (!r.kept(cut, v, i)) return 0.0;
-          const double w = r.weight(v);
-          return w >= floor_w ? w : 0.0;
-        },
-        [&](double total) { return (double)u * total; });
+    if (!drawn) {
+      const double floor_w = (double)min_p;
+      token = r.ordered_find(
+          [&](float v, int i) {
+            if (!r.kept(cut, v, i)) return 0.0;
+            const double w = r.weight(v);
+            return w >= floor_w ? w : 0.0;
+          },
+          [&](double total) { return (double)u * total; });
+      if (r.lane) token = -1;
+    }
   }
-  if (token != -1 && r.lane == 0 && (token >= 0 || threadIdx.x == 0)) p.out[row] = token >= 0 ? token : -1;
+  if (token >= 0) p.out[row] = token;
   r.cluster_barrier();  // no CTA leaves while its shared memory may still be read
   pdl_launch_dependents();
 }
@@ -506,7 +892,7 @@ static int launch(const Params &p, int64_t rows, size_t smem, cudaStream_t st) {
   int dev = 0;
   HEXB_CUDA_OK(cudaGetDevice(&dev));
   if (!once.is_done(dev)) {
-    HEXB_CUDA_OK(cudaFuncSetAttribute(sample_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, 196 * 1024));
+    HEXB_CUDA_OK(cudaFuncSetAttribute(sample_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
     once.mark(dev);
   }
   cudaLaunchConfig_t cfg = {};
@@ -530,13 +916,14 @@ template <typename T>
 static int dispatch(Params p, int64_t rows, cudaStream_t st) {
   DeviceInfo di;
   if (int e = current_device(&di)) return e;
-  // CTAs of a row: enough that a slice is at most 16384 logits, up to the 8 of a portable cluster.
+  // CTAs of a row: one when the rows alone fill the GPU (its row stays in L2), else enough to spread the row over idle SMs,
+  // up to the 8 of a portable cluster and down to slices of 4096 logits.
   int c = 1;
-  while (c < MAXC && (p.V + c - 1) / c > 16384) c *= 2;
+  while (c < MAXC && rows * c * 2 <= di.sm_count && (p.V + c - 1) / c > 4096) c *= 2;
   p.slice = ((p.V + c - 1) / c + 7) / 8 * 8;
-  const size_t bytes = (size_t)p.slice * sizeof(T) + 32;
-  p.resident = bytes <= 192 * 1024;
-  const size_t smem = p.resident ? bytes : 0;
+  const size_t fixed = (sizeof(Shared) + 15) / 16 * 16, bytes = (size_t)p.slice * sizeof(T) + 32;
+  p.resident = c > 1 && fixed + bytes <= 220 * 1024;
+  const size_t smem = fixed + (p.resident ? bytes : 0);
   switch (c) {
     case 1: return launch<T, 1>(p, rows, smem, st);
     case 2: return launch<T, 2>(p, rows, smem, st);
