@@ -34,7 +34,8 @@ constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int NB = 2048;           // histogram bins
 constexpr int CAP = 4096;          // list entries
 constexpr int MAXC = 8;
-constexpr int kLevels = 16;        // of the exponential's table
+constexpr int kLevelBits = 7, kLevels = 1 << kLevelBits;  // of the exponential's table
+constexpr uint32_t kNoCut = 0x007fffffu;  // key of -inf
 
 struct Params {
   const void *x;
@@ -57,10 +58,11 @@ __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 // A finite float in 64 bits by integer operations (the conversion instruction runs at an eighth of the rate); zero and
-// subnormal numbers come out below 2^-126, which changes no sum here.
+// subnormal numbers come out below 2^-126, which changes no sum here.  T: the type the value was widened from.
+template <typename T>
 __device__ __forceinline__ double widen(float x) {
   const uint32_t b = __float_as_uint(x), mag = b & 0x7fffffffu;
-  return __hiloint2double((int)((b & 0x80000000u) | ((mag >> 3) + 0x38000000u)), (int)(mag << 29));
+  return __hiloint2double((int)((b & 0x80000000u) | ((mag >> 3) + 0x38000000u)), sizeof(T) == 2 ? 0 : (int)(mag << 29));
 }
 
 // What is kept so far: keys above `key`, and of those equal to it the indices up to `index`.
@@ -112,6 +114,7 @@ __device__ __forceinline__ uint32_t add_cluster_u32(uint32_t addr, uint32_t v) {
 
 template <typename T, int C>
 struct Row {
+  static constexpr int E = Vec16<T>::N;
   const Params &p;
   Shared &s;
   const T *data;          // the slice: shared memory, or global
@@ -121,7 +124,7 @@ struct Row {
   int first;              // row index of slice element 0
   float m, f_bin;         // maximum; bins per unit of value
   double scale, offset;   // (x, T) -> kLevels * log2 of the weight
-  float scale32;
+  float scale32, v_min;
   int flip;
 
   __device__ Row(const Params &p_, Shared &s_) : p(p_), s(s_), flip(0) {}
@@ -134,40 +137,61 @@ struct Row {
     const uint32_t l = tc::smem_u32(a);
     return C > 1 ? tc::map_to_rank(l, (uint32_t)r) : l;
   }
-  // 2^(y / kLevels) for y = kLevels * log2(e) * (v - m) / T <= 0, in 64 bits: y = k + f, |f| <= 1/2; 2^(k / kLevels) from the table
-  // and the exponent, 2^(f / kLevels) by its Taylor series (degree 5: the next term is below 0.0217^6 / 720 = 2e-13).
+  // exp((v - m) / T) in 64 bits: y = kLevels * log2(e) * (v - m) / T = k + f, |f| <= 1/2; 2^(k / kLevels) from the table and the
+  // exponent, 2^(f / kLevels) by its Taylor series (degree 3: the next term is below 0.0028^4 / 24 = 3e-12, two
+  // orders under what the sums need).  Below v_min the weight, 2^-1000, counts as 0.
   __device__ __forceinline__ double weight(float v) const {
-    if (v == m) return 1.0;
-    const double y = fma(widen(v), scale, offset);
-    if (!(y > -16000.0)) return 0.0;                 // 2^-1000
+    const double y = fma(widen<T>(v), scale, offset);
     const double magic = 6755399441055744.0;         // 1.5 * 2^52: the sum's low word is the rounded y
     const double z = y + magic;
-    const int k = __double2loint(z);
+    const int k = -__double2loint(z);
     const double f = y - (z - magic);
     constexpr double L = 0.693147180559945309417 / kLevels;
-    double r = L * L * L * L * L / 120.0;
-    r = fma(r, f, L * L * L * L / 24.0);
-    r = fma(r, f, L * L * L / 6.0);
-    r = fma(r, f, L * L / 2.0);
+    double r = fma(L * L * L / 6.0, f, L * L / 2.0);
     r = fma(r, f, L);
     r = fma(r, f, 1.0);
-    const double w = r * s.table[-k & (kLevels - 1)];
-    return __hiloint2double(__double2hiint(w) - ((-k) / kLevels << 20), __double2loint(w));
+    const double w = r * s.table[k & (kLevels - 1)];
+    const double e = __hiloint2double(__double2hiint(w) - ((k & ~(kLevels - 1)) << (20 - kLevelBits)), __double2loint(w));
+    return v < v_min ? 0.0 : e;
+  }
+  // Weights of the elements of one vector that the cut keeps, 0 for the others.  Without a branch an element, so that
+  // the chains of a vector's elements overlap (with one, a pass over 256 rows of 128000 took 121 us).
+  __device__ __forceinline__ void weigh(const Cut &c, const float (&x)[E], int i0, double (&w)[E]) const {
+    const float at = value_of(c.key), low = fmaxf(at, v_min);
+    float top = x[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
+    if (top < low) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) w[e] = 0.0;
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const bool out = x[e] < low || (x[e] == at && i0 + e > c.index);
+      const double v = weight(x[e]);
+      w[e] = out ? 0.0 : v;
+    }
+  }
+  // Lowest key whose weight is at least min_p: weights do not fall as keys rise.
+  __device__ uint32_t min_p_key(float min_p) const {
+    uint32_t lo = 0x00800000u, hi = key_of(m);
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (weight(value_of(mid)) >= (double)min_p) hi = mid;
+      else lo = mid + 1;
+    }
+    return lo;
   }
   __device__ __forceinline__ bool kept(const Cut &c, float v, int i) const {
-    const uint32_t k = key_of(v);
-    return v > -INFINITY && (k > c.key || (k == c.key && i <= c.index));
+    const float at = value_of(c.key);                // (-inf for no cut: it keeps no -inf either)
+    return v > at || (v == at && i <= c.index && at > -INFINITY);
   }
-  __device__ __forceinline__ int bin_of(float v) const {
-    const float d = v == m ? 0.0f : m - v;
-    return (int)fminf(d * f_bin, (float)(NB - 1));
-  }
-  // f(value, row index) for the elements of vector v (NaN arrives as -inf)
-  template <typename F>
-  __device__ __forceinline__ void vector(int v, F &&f) const {
-    constexpr int E = Vec16<T>::N;
+  // Does not fall as v falls (an infinite maximum: one bin for all).
+  __device__ __forceinline__ int bin_of(float v) const { return (int)fminf((m - v) * f_bin, (float)(NB - 1)); }
+  // The elements of vector v, and the row index of the first.  NaN, and places outside the slice, come as -inf.
+  __device__ __forceinline__ int vector(int v, float (&x)[E]) const {
     const int i = v * E - shift;
-    float x[E];
     if (i >= 0 && i + E <= n) {
       Vec16<T> q;
       q.raw = *reinterpret_cast<const decltype(q.raw) *>(data + i);
@@ -177,13 +201,18 @@ struct Row {
       for (int e = 0; e < E; ++e) x[e] = i + e >= 0 && i + e < n ? to_f32<T>(data[i + e]) : -INFINITY;
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) f(x[e] != x[e] ? -INFINITY : x[e], first + i + e);
+    for (int e = 0; e < E; ++e) x[e] = fmaxf(x[e], -INFINITY);
+    return first + i;
   }
-  // f for every element of this warp's part, and -inf for some places beside it
+  // f(values, row index of the first) for every vector of this warp's part
   template <typename F>
   __device__ __forceinline__ void each(F &&f) const {
 #pragma unroll 2
-    for (int v = v0 + lane; v < v1; v += 32) vector(v, f);
+    for (int v = v0 + lane; v < v1; v += 32) {
+      float x[E];
+      const int i = vector(v, x);
+      f(x, i);
+    }
   }
 
   // Sum of one 64-bit value per thread over the cluster: lanes, warps in order, CTAs in order.  Also leaves the
@@ -215,7 +244,12 @@ struct Row {
   template <typename F, typename G>
   __device__ int ordered_find(F &&f, G &&target) {
     double v = 0.0;
-    each([&](float x, int i) { v += f(x, i); });
+    each([&](const float (&x)[E], int i) {
+      double w[E];
+      f(x, i, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) v += w[e];
+    });
     double cta[C];
     const double total = cluster_total(v, cta);
     if (!(total > 0.0)) return -1;
@@ -249,7 +283,6 @@ struct Row {
     __syncthreads();
     if (warp != s.winner) return -1;
     // a lane's vector first, then the element in it
-    constexpr int E = Vec16<T>::N;
     double run = s.rel;
     int last = -1;
     for (int vb = v0; vb < v1; vb += 32) {
@@ -259,12 +292,11 @@ struct Row {
 #pragma unroll
       for (int e = 0; e < E; ++e) own[e] = 0.0;
       if (vv < v1) {
-        int e = 0;
-        vector(vv, [&](float x, int i) {
-          own[e++] = f(x, i);
-          sum += own[e - 1];
-        });
-        at = first + vv * E - shift;
+        float x[E];
+        at = vector(vv, x);
+        f(x, at, own);
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum += own[e];
       }
       double incl = sum;
 #pragma unroll
@@ -335,13 +367,15 @@ struct Row {
   // Leaves: b_k, before_k  bin of the k-th logit and the count before it
   //         b_p            guess of the bin where p of the mass (of what top-k leaves) is reached
   //         b_last         the last bin that the list needs, n_last logits up to it; guessed: b_p set it
-  //         n_first, n_guess   logits before bin b_p - 3, and up to bin b_p + 3
+  //         n_first, n_guess   logits before bin b_p - 1, and up to bin b_p + 1
   __device__ void plan(const Cut &in, int top_k, float top_p, float min_p, float lowest) {
     const float range = fminf(m - lowest, 32.0f);
     f_bin = range > 1e-20f ? (float)NB / range : 0.0f;
     clear(false);
-    each([&](float v, int) {
-      if (v > -INFINITY) atomicAdd(&s.count[bin_of(v)], 1u);
+    each([&](const float (&x)[E], int) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (x[e] > -INFINITY) atomicAdd(&s.count[bin_of(x[e])], 1u);
     });
     if (threadIdx.x == 0) {
       s.b_k = s.b_p = NB - 1;
@@ -395,14 +429,14 @@ struct Row {
       limit = min(limit, (int)fminf(d * f_bin, (float)(NB - 4)) + 2);
     }
     // the mass that top-p takes its share of is top-k's, if there is one: then the list has to hold that
-    const int last = top_p < 1.0f ? (top_k > 0 ? b_k : min(limit, s.b_p + 3)) : limit;
+    const int last = top_p < 1.0f ? (top_k > 0 ? b_k : min(limit, s.b_p + 1)) : limit;
     u64 e = before;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (b0 + i == s.b_p - 3) s.n_first = (int)e;
+      if (b0 + i == s.b_p - 1) s.n_first = (int)e;
       e += c[i];
       if (b0 + i == last) s.n_last = (int)e;
-      if (b0 + i == min(s.b_p + 3, NB - 1)) s.n_guess = (int)e;
+      if (b0 + i == min(s.b_p + 1, NB - 1)) s.n_guess = (int)e;
     }
     if (threadIdx.x == 0) {
       s.b_last = last;
@@ -429,23 +463,33 @@ struct Row {
       else s.list[at] = entry;
     }
   }
-  // f(take, value, index) by whole warps
+  // f(values, row index of the first), by whole warps
   template <typename F>
   __device__ __forceinline__ void each_warp(F &&f) {
-    constexpr int E = Vec16<T>::N;
     for (int vb = v0; vb < v1; vb += 32) {
       const int vv = vb + lane;
       float x[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) x[e] = -INFINITY;
       int at = 0;
-      if (vv < v1) {
-        int e = 0;
-        vector(vv, [&](float v, int) { x[e++] = v; });
-        at = first + vv * E - shift;
-      }
+      if (vv < v1) at = vector(vv, x);
+      f(x, at);
+    }
+  }
+  // Appends the elements in bins [lo, hi] that the cut keeps.
+  __device__ __forceinline__ void append(const Cut &c, int lo, int hi, const float (&x)[E], int i0) {
+    float top = x[0], low = x[0];
 #pragma unroll
-      for (int e = 0; e < E; ++e) f(x[e], at + e);
+    for (int e = 1; e < E; ++e) {
+      top = fmaxf(top, x[e]);
+      low = fminf(low, x[e]);
+    }
+    // most vectors hold none
+    if (!__any_sync(0xffffffffu, top > -INFINITY && bin_of(top) <= hi && (lo <= 0 || bin_of(low) >= lo))) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int b = x[e] > -INFINITY ? bin_of(x[e]) : NB;
+      append(b >= lo && b <= hi && kept(c, x[e], i0 + e), x[e], i0 + e);
     }
   }
   // Descending bitonic sort of the list (all threads of CTA 0).
@@ -464,8 +508,11 @@ struct Row {
             a[hi] = x;
           }
         }
-        __syncthreads();
+        // up to j = 32 a warp's pairs lie in 64 entries that only it touches
+        if (j > 32 || j == 1 && k >= 64) __syncthreads();
+        else __syncwarp();
       }
+    __syncthreads();
   }
   // s.mass[i] <- sum of the weights of list entries 0 .. i (CTA 0).  Fixed order: eight consecutive entries a thread.
   __device__ void accumulate(int n) {
@@ -521,9 +568,15 @@ struct Row {
     list_reset();
     double sum = 0.0, cta[C];
     const bool total_needed = top_p < 1.0f && top_k <= 0;
-    each_warp([&](float v, int i) {
-      append(v > -INFINITY && bin_of(v) <= last, v, i);
-      if (total_needed && v > -INFINITY) sum += weight(v);
+    const Cut all = {kNoCut, 0x7fffffff};
+    each_warp([&](const float (&x)[E], int i) {
+      append(all, 0, last, x, i);
+      if (total_needed) {
+        double w[E];
+        weigh(all, x, i, w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum += w[e];
+      }
     });
     double total = 0.0;
     if (total_needed) total = cluster_total(sum, cta);
@@ -578,7 +631,8 @@ struct Row {
     const int b = s.b_k;
     const int rank_in = top_k - (int)s.before_k;     // 1 ..
     list_reset();
-    each_warp([&](float v, int i) { append(v > -INFINITY && bin_of(v) == b, v, i); });
+    const Cut all = {kNoCut, 0x7fffffff};
+    each_warp([&](const float (&x)[E], int i) { append(all, b, b, x, i); });
     cluster_barrier();
     if (rank == 0) {
       const int n = (int)min(s.n, (uint32_t)CAP);
@@ -592,19 +646,19 @@ struct Row {
     }
     return broadcast(cut);
   }
-  // p of the mass: guessed to lie in bins [b_p - 3, b_p + 3].
+  // p of the mass: guessed to lie in bin b_p or beside it.
   __device__ bool refine_p(Cut &cut, float top_p) {
-    const int lo = s.b_p - 3, hi = s.b_p + 3;
+    const int lo = s.b_p - 1, hi = s.b_p + 1;
     list_reset();
     double sum = 0.0, above = 0.0, cta[C];
-    each_warp([&](float v, int i) {
-      const bool k = kept(cut, v, i);
-      const int b = k ? bin_of(v) : NB;
-      append(b >= lo && b <= hi, v, i);
-      if (k) {
-        const double w = weight(v);
-        sum += w;
-        if (b < lo) above += w;
+    each_warp([&](const float (&x)[E], int i) {
+      append(cut, lo, hi, x, i);
+      double w[E];
+      weigh(cut, x, i, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        sum += w[e];
+        above += x[e] > -INFINITY && bin_of(x[e]) < lo ? w[e] : 0.0;
       }
     });
     const double total = cluster_total(sum, cta);
@@ -685,10 +739,10 @@ struct Row {
   // The cut of top-k (MASS false: `need` elements) or top-p (MASS true: `need` units of mass; unit = 1 / units): bins of
   // keys, narrowed until a bin is one key.
   template <bool MASS>
-  __device__ Cut descend(const Cut &in, double need, double units, float lowest) {
+  __device__ Cut descend(const Cut &in, double need, double units) {
     constexpr int KS = sizeof(T) == 2 ? 13 : 0;  // a widened fp16 value leaves the low 13 bits of its key alone
     uint32_t *hi_words = reinterpret_cast<uint32_t *>(s.list), *lo_words = hi_words + NB;
-    uint32_t lo = key_of(lowest), hi = key_of(m);
+    uint32_t lo = 0x00800000u, hi = key_of(m);       // all finite values up to the maximum
     u64 before = 0;
     while (true) {
       const uint32_t span = (hi >> KS) - (lo >> KS);   // keys - 1
@@ -696,13 +750,15 @@ struct Row {
       while ((span >> sh) >= (uint32_t)NB) ++sh;
       __syncthreads();
       clear(MASS);
-      each([&](float v, int i) {
-        const uint32_t k = key_of(v);
-        if (k >= lo && k <= hi && kept(in, v, i)) {
+      each([&](const float (&x)[E], int i) {
+#pragma unroll 1
+        for (int e = 0; e < E; ++e) {
+          const uint32_t k = key_of(x[e]);
+          if (k < lo || k > hi || !kept(in, x[e], i + e)) continue;
           const uint32_t b = ((hi >> KS) - (k >> KS)) >> sh;
           atomicAdd(&s.count[b], 1u);
           if (MASS) {
-            const u64 q = __double2ull_rn(weight(v) * units);
+            const u64 q = __double2ull_rn(weight(x[e]) * units);
             atomicAdd(&hi_words[b], (uint32_t)(q >> 14));
             atomicAdd(&lo_words[b], (uint32_t)(q & 16383u));
           }
@@ -731,7 +787,11 @@ struct Row {
 
   // Row index of the t-th kept element with key k.
   __device__ int tie_index(const Cut &in, uint32_t k, double t) {
-    const int i = ordered_find([&](float v, int j) { return key_of(v) == k && kept(in, v, j) ? 1.0 : 0.0; },
+    const int i = ordered_find(
+        [&](const float (&x)[E], int j, double (&w)[E]) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) w[e] = key_of(x[e]) == k && kept(in, x[e], j + e) ? 1.0 : 0.0;
+        },
                                [&](double) { return t - 0.5; });
     if (i >= 0 && lane == 0)
       for (int r = 0; r < C; ++r) st_cluster_u32(peer(&s.found_index, r), (uint32_t)i);
@@ -756,7 +816,7 @@ sample_kernel(const Params p) {
   r.first = r.rank * p.slice;
   r.n = max(0, min(p.slice, p.V - r.first));
   const T *src = static_cast<const T *>(p.x) + (int64_t)row * p.row_stride + r.first;
-  if (threadIdx.x < kLevels) s.table[threadIdx.x] = exp2(-(double)threadIdx.x / kLevels);
+  for (int i = threadIdx.x; i < kLevels; i += THREADS) s.table[i] = exp2(-(double)i / kLevels);
   // the peers' shared memory may be written once every CTA of the cluster has started
   if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   pdl_wait();
@@ -772,15 +832,14 @@ sample_kernel(const Params p) {
   r.v1 = min(r.v0 + per, vecs);
   r.data = src;
   T *copy = reinterpret_cast<T *>(dyn + (sizeof(Shared) + 15) / 16 * 16) + r.shift;  // as aligned as the source
-  u64 best = 0;
-  float mn = INFINITY;
-#pragma unroll 4
-  for (int v = r.v0 + r.lane; v < r.v1; v += 32) {
+  // maximum with its place, and the minimum of a sample (each lane's first vector) for the width of the bins
+  float top = -INFINITY, mn = INFINITY;
+  int top_v = 0;
+  auto load = [&](int v, float (&x)[E]) {
     const int i = v * E - r.shift;
-    float x[E];
     if (i >= 0 && i + E <= r.n) {
       Vec16<T> q;
-      q.raw = *reinterpret_cast<const decltype(q.raw) *>(src + i);
+      q.raw = ld_stream_as<decltype(q.raw)>(src + i);
       if (p.resident) *reinterpret_cast<decltype(q.raw) *>(copy + i) = q.raw;
       q.unpack(x);
     } else {
@@ -794,21 +853,31 @@ sample_kernel(const Params p) {
         }
       }
     }
-    float top = -INFINITY;
+  };
+#pragma unroll 4
+  for (int v = r.v0 + r.lane; v < r.v1; v += 32) {
+    float x[E];
+    load(v, x);
+    float t = x[0];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (x[e] > -INFINITY) {  // neither NaN nor -inf
-        top = fmaxf(top, x[e]);
-        mn = fminf(mn, x[e]);
-      }
+    for (int e = 1; e < E; ++e) t = fmaxf(t, x[e]);   // NaN loses
+    if (t > top) {                                    // a lane's places rise: the first of equal ones stays
+      top = t;
+      top_v = v;
     }
-    if (top > -INFINITY && (best == 0 || key_of(top) > (uint32_t)(best >> 32))) {  // a lane's indices rise: the first stays
-      int at = 0;
+    if (v == r.v0 + r.lane) {
 #pragma unroll
-      for (int e = E - 1; e >= 0; --e)
-        if (x[e] == top) at = e;
-      best = (u64)key_of(top) << 32 | (uint32_t)~(r.first + i + at);
+      for (int e = 0; e < E; ++e)
+        if (x[e] > -INFINITY) mn = fminf(mn, x[e]);
     }
+  }
+  u64 best = 0;
+  if (top > -INFINITY) {
+    const int i = top_v * E - r.shift;
+    int at = 0;
+    for (int e = E - 1; e >= 0; --e)
+      if (i + e >= 0 && i + e < r.n && to_f32<T>(src[i + e]) == top) at = e;
+    best = (u64)key_of(top) << 32 | (uint32_t)~(r.first + i + at);
   }
   if (p.resident) r.data = copy;
 #pragma unroll
@@ -849,7 +918,12 @@ sample_kernel(const Params p) {
     r.offset = -(double)r.m * r.scale;
     r.scale32 = (float)c;
     if (top_k >= p.V) top_k = 0;
-    Cut cut = {0u, 0x7fffffff};
+    r.v_min = (float)((double)r.m - 1000.0 / c);
+    if (r.m == INFINITY) {
+      r.scale = r.offset = 0.0;   // its own weight is 1,
+      r.v_min = INFINITY;         // any other 0
+    }
+    Cut cut = {kNoCut, 0x7fffffff};
     bool drawn = false;
     if (top_k > 0 || top_p < 1.0f) {
       r.plan(cut, top_k, top_p, min_p, mn);
@@ -860,24 +934,27 @@ sample_kernel(const Params p) {
       }
       if (!drawn) {
         const int n_p = s.n_guess - s.n_first;   // logits around the guess
-        if (top_k > 0 && !r.refine_k(cut, top_k)) cut = r.template descend<false>(cut, (double)top_k, 0.0, mn);
+        if (top_k > 0 && !r.refine_k(cut, top_k)) cut = r.template descend<false>(cut, (double)top_k, 0.0);
         if (top_p < 1.0f && !(n_p <= CAP && r.refine_p(cut, top_p))) {
           double part = 0.0, cta[C];
-          r.each([&](float v, int i) { if (r.kept(cut, v, i)) part += r.weight(v); });
+          r.each([&](const float (&x)[E], int i) {
+            double w[E];
+            r.weigh(cut, x, i, w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) part += w[e];
+          });
           const double units = 17592186044416.0 / r.cluster_total(part, cta);  // 2^44 in all
-          cut = r.template descend<true>(cut, fmax((double)top_p * 17592186044416.0, 1.0), units, mn);
+          cut = r.template descend<true>(cut, fmax((double)top_p * 17592186044416.0, 1.0), units);
         }
       }
     }
     if (!drawn) {
-      const double floor_w = (double)min_p;
-      token = r.ordered_find(
-          [&](float v, int i) {
-            if (!r.kept(cut, v, i)) return 0.0;
-            const double w = r.weight(v);
-            return w >= floor_w ? w : 0.0;
-          },
-          [&](double total) { return (double)u * total; });
+      if (min_p > 0.0f) {
+        const uint32_t k = r.min_p_key(min_p);
+        if (k > cut.key) cut = {k, 0x7fffffff};
+      }
+      token = r.ordered_find([&](const float (&x)[E], int i, double (&w)[E]) { r.weigh(cut, x, i, w); },
+                             [&](double total) { return (double)u * total; });
       if (r.lane) token = -1;
     }
   }
