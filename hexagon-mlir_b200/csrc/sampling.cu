@@ -57,14 +57,6 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
-// A finite float in 64 bits by integer operations (the conversion instruction runs at an eighth of the rate); zero and
-// subnormal numbers come out below 2^-126, which changes no sum here.  T: the type the value was widened from.
-template <typename T>
-__device__ __forceinline__ double widen(float x) {
-  const uint32_t b = __float_as_uint(x), mag = b & 0x7fffffffu;
-  return __hiloint2double((int)((b & 0x80000000u) | ((mag >> 3) + 0x38000000u)), sizeof(T) == 2 ? 0 : (int)(mag << 29));
-}
-
 // What is kept so far: keys above `key`, and of those equal to it the indices up to `index`.
 struct Cut {
   uint32_t key;
@@ -125,9 +117,10 @@ struct Row {
   float m, f_bin;         // maximum; bins per unit of value
   double scale, offset;   // (x, T) -> kLevels * log2 of the weight
   float scale32, v_min;
+  bool infinite;          // the maximum is: the elements come as the largest finite value, or as -inf
   int flip;
 
-  __device__ Row(const Params &p_, Shared &s_) : p(p_), s(s_), flip(0) {}
+  __device__ Row(const Params &p_, Shared &s_) : p(p_), s(s_), infinite(false), flip(0) {}
 
   __device__ __forceinline__ void cluster_barrier() {
     if (C > 1) tc::cluster_sync_all();
@@ -140,8 +133,9 @@ struct Row {
   // exp((v - m) / T) in 64 bits: y = kLevels * log2(e) * (v - m) / T = k + f, |f| <= 1/2; 2^(k / kLevels) from the table and the
   // exponent, 2^(f / kLevels) by its Taylor series (degree 3: the next term is below 0.0028^4 / 24 = 3e-12, two
   // orders under what the sums need).  Below v_min the weight, 2^-1000, counts as 0.
-  __device__ __forceinline__ double weight(float v) const {
-    const double y = fma(widen<T>(v), scale, offset);
+  __device__ __forceinline__ double weight(float v) const { return v < v_min ? 0.0 : weight_above(v); }
+  __device__ __forceinline__ double weight_above(float v) const {   // v >= v_min
+    const double y = fma((double)v, scale, offset);
     const double magic = 6755399441055744.0;         // 1.5 * 2^52: the sum's low word is the rounded y
     const double z = y + magic;
     const int k = -__double2loint(z);
@@ -151,8 +145,7 @@ struct Row {
     r = fma(r, f, L);
     r = fma(r, f, 1.0);
     const double w = r * s.table[k & (kLevels - 1)];
-    const double e = __hiloint2double(__double2hiint(w) - ((k & ~(kLevels - 1)) << (20 - kLevelBits)), __double2loint(w));
-    return v < v_min ? 0.0 : e;
+    return __hiloint2double(__double2hiint(w) - ((k & ~(kLevels - 1)) << (20 - kLevelBits)), __double2loint(w));
   }
   // Weights of the elements of one vector that the cut keeps, 0 for the others.  Without a branch an element, so that
   // the chains of a vector's elements overlap (with one, a pass over 256 rows of 128000 took 121 us).
@@ -168,9 +161,13 @@ struct Row {
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const bool out = x[e] < low || (x[e] == at && i0 + e > c.index);
-      const double v = weight(x[e]);
-      w[e] = out ? 0.0 : v;
+      const double v = weight_above(x[e]);
+      w[e] = x[e] < low ? 0.0 : v;
+    }
+    if (i0 + E - 1 > c.index) {                       // the cut runs through equal logits, behind the last that stays
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (x[e] == at && i0 + e > c.index) w[e] = 0.0;
     }
   }
   // Lowest key whose weight is at least min_p: weights do not fall as keys rise.
@@ -187,7 +184,7 @@ struct Row {
     const float at = value_of(c.key);                // (-inf for no cut: it keeps no -inf either)
     return v > at || (v == at && i <= c.index && at > -INFINITY);
   }
-  // Does not fall as v falls (an infinite maximum: one bin for all).
+  // Does not fall as v falls.
   __device__ __forceinline__ int bin_of(float v) const { return (int)fminf((m - v) * f_bin, (float)(NB - 1)); }
   // The elements of vector v, and the row index of the first.  NaN, and places outside the slice, come as -inf.
   __device__ __forceinline__ int vector(int v, float (&x)[E]) const {
@@ -202,6 +199,10 @@ struct Row {
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = fmaxf(x[e], -INFINITY);
+    if (infinite) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = x[e] == INFINITY ? m : -INFINITY;
+    }
     return first + i;
   }
   // f(values, row index of the first) for every vector of this warp's part
@@ -266,64 +267,77 @@ struct Row {
       excl += cta[r];
     }
     if (win != rank) return -1;
-    if (threadIdx.x == 0) {
-      double e = win_excl;
-      int w_win = -1;
-      double w_excl = 0.0;
-      for (int w = 0; w < WARPS; ++w) {
-        if (s.warp_sum[w] > 0.0 && (w_win < 0 || e <= t)) {
-          w_win = w;
-          w_excl = e;
+    // The warp whose part holds it; then that part is dealt to all warps, until a part is one vector a lane.  (One warp
+    // alone over its part of 128000 logits: 20 us.)
+    int lo = 0, hi = (n + shift + E - 1) / E;
+    double base = win_excl;
+    while (true) {
+      const int len = (hi - lo + WARPS - 1) / WARPS;
+      if (threadIdx.x == 0) {
+        double e = base;
+        s.winner = -1;
+        for (int w = 0; w < WARPS; ++w) {
+          if (s.warp_sum[w] > 0.0 && (s.winner < 0 || e <= t)) {
+            s.winner = w;
+            s.rel = e;
+          }
+          e += s.warp_sum[w];
         }
-        e += s.warp_sum[w];
       }
-      s.winner = w_win;
-      s.rel = w_excl;
-    }
-    __syncthreads();
-    if (warp != s.winner) return -1;
-    // a lane's vector first, then the element in it
-    double run = s.rel;
-    int last = -1;
-    for (int vb = v0; vb < v1; vb += 32) {
-      const int vv = vb + lane;
-      double own[E], sum = 0.0;
-      int at = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) own[e] = 0.0;
-      if (vv < v1) {
+      __syncthreads();
+      lo = min(lo + s.winner * len, hi);
+      hi = min(lo + len, hi);
+      base = s.rel;
+      if (hi - lo <= 32) break;
+      const int part = (hi - lo + WARPS - 1) / WARPS, a = min(lo + warp * part, hi), b = min(a + part, hi);
+      double sum = 0.0;
+      for (int vv = a + lane; vv < b; vv += 32) {
         float x[E];
-        at = vector(vv, x);
-        f(x, at, own);
+        double w[E];
+        const int i = vector(vv, x);
+        f(x, i, w);
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum += own[e];
+        for (int e = 0; e < E; ++e) sum += w[e];
       }
-      double incl = sum;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
-      }
-      const unsigned any = __ballot_sync(0xffffffffu, sum > 0.0);
-      const unsigned over = __ballot_sync(0xffffffffu, sum > 0.0 && run + incl > t);
-      // the lane that crosses, or the last that holds anything: its elements in order
-      const int from = over ? __ffs(over) - 1 : any ? 31 - __clz(any) : -1;
-      int mine = -1;
-      if (lane == from) {
-        double c = run + (incl - sum);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          c += own[e];
-          if (own[e] > 0.0 && (mine < 0 || !(c - own[e] > t))) mine = at + e;
-        }
-      }
-      if (from >= 0) {
-        last = __shfl_sync(0xffffffffu, mine, from);
-        if (over) return last;
-      }
-      run += __shfl_sync(0xffffffffu, incl, 31);
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      __syncthreads();
+      if (lane == 0) s.warp_sum[warp] = sum;
+      __syncthreads();
     }
-    return last;  // the sums of the scan and of the lanes may round apart: the last one then
+    if (warp) return -1;
+    // a lane's vector first, then the element in it
+    double own[E], sum = 0.0;
+    int at = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) own[e] = 0.0;
+    if (lo + lane < hi) {
+      float x[E];
+      at = vector(lo + lane, x);
+      f(x, at, own);
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum += own[e];
+    }
+    double incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const unsigned any = __ballot_sync(0xffffffffu, sum > 0.0);
+    const unsigned over = __ballot_sync(0xffffffffu, sum > 0.0 && base + incl > t);
+    // the lane that crosses, or (sums of scan and lanes may round apart) the last that holds anything
+    const int from = over ? __ffs(over) - 1 : 31 - __clz(any);
+    int mine = -1;
+    if (lane == from) {
+      double c = base + (incl - sum);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (own[e] > 0.0 && (mine < 0 || !(c > t))) mine = at + e;
+        c += own[e];
+      }
+    }
+    return __shfl_sync(0xffffffffu, mine, from);
   }
 
   __device__ void clear(bool mass) {
@@ -919,9 +933,11 @@ sample_kernel(const Params p) {
     r.scale32 = (float)c;
     if (top_k >= p.V) top_k = 0;
     r.v_min = (float)((double)r.m - 1000.0 / c);
-    if (r.m == INFINITY) {
-      r.scale = r.offset = 0.0;   // its own weight is 1,
-      r.v_min = INFINITY;         // any other 0
+    if (r.m == INFINITY) {        // weight 1 for its like, 0 for any other: as if both were the largest finite value
+      r.infinite = true;
+      r.m = 3.402823466e38f;
+      r.scale = r.offset = 0.0;
+      r.v_min = r.m;
     }
     Cut cut = {kNoCut, 0x7fffffff};
     bool drawn = false;
