@@ -107,6 +107,7 @@ __device__ __forceinline__ uint32_t add_cluster_u32(uint32_t addr, uint32_t v) {
 template <typename T, int C>
 struct Row {
   static constexpr int E = Vec16<T>::N;
+  using Raw = decltype(Vec16<T>::raw);
   const Params &p;
   Shared &s;
   const T *data;          // the slice: shared memory, or global
@@ -184,14 +185,27 @@ struct Row {
     const float at = value_of(c.key);                // (-inf for no cut: it keeps no -inf either)
     return v > at || (v == at && i <= c.index && at > -INFINITY);
   }
-  // Does not fall as v falls.
-  __device__ __forceinline__ int bin_of(float v) const { return (int)fminf((m - v) * f_bin, (float)(NB - 1)); }
+  // Does not fall as v falls.  (bin_of(v) < b, for b < NB, is depth(v) < b.)
+  __device__ __forceinline__ float depth(float v) const { return (m - v) * f_bin; }
+  __device__ __forceinline__ int bin_of(float v) const { return (int)fminf(depth(v), (float)(NB - 1)); }
   // The elements of vector v, and the row index of the first.  NaN, and places outside the slice, come as -inf.
   __device__ __forceinline__ int vector(int v, float (&x)[E]) const {
+    Raw raw;
+    return expand(v, fetch(v, vectors(), raw), raw, x);
+  }
+  __device__ __forceinline__ int vectors() const { return (n + shift + E - 1) / E; }
+  // Whole vectors below `end` are requested here, so that several are under way; others are read element by element.
+  __device__ __forceinline__ bool fetch(int v, int end, Raw &raw) const {
     const int i = v * E - shift;
-    if (i >= 0 && i + E <= n) {
+    const bool whole = v < end && i >= 0 && i + E <= n;
+    if (whole) raw = *reinterpret_cast<const Raw *>(data + i);
+    return whole;
+  }
+  __device__ __forceinline__ int expand(int v, bool whole, const Raw &raw, float (&x)[E]) const {
+    const int i = v * E - shift;
+    if (whole) {
       Vec16<T> q;
-      q.raw = *reinterpret_cast<const decltype(q.raw) *>(data + i);
+      q.raw = raw;
       q.unpack(x);
     } else {
 #pragma unroll
@@ -205,14 +219,35 @@ struct Row {
     }
     return first + i;
   }
-  // f(values, row index of the first) for every vector of this warp's part
+  // f(values, row index of the first) for every vector of this warp's part, by whole warps (lanes without a vector get -inf)
   template <typename F>
   __device__ __forceinline__ void each(F &&f) const {
-#pragma unroll 2
-    for (int v = v0 + lane; v < v1; v += 32) {
-      float x[E];
-      const int i = vector(v, x);
-      f(x, i);
+    constexpr int AHEAD = 4;
+    for (int vb = v0; vb < v1; vb += 32 * AHEAD) {
+      Raw raw[AHEAD];
+      bool whole[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) whole[j] = fetch(vb + j * 32 + lane, v1, raw[j]);
+#pragma unroll 1
+      for (int j = 0; j < AHEAD; ++j) {
+        if (vb + j * 32 >= v1) break;
+        const int v = vb + j * 32 + lane;
+        float x[E];
+        int at = 0;
+        if (v < v1) {
+          at = expand(v, whole[0], raw[0], x);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[e] = -INFINITY;
+        }
+        f(x, at);
+        // the next one moves up: one copy of f's code
+#pragma unroll
+        for (int k = 0; k + 1 < AHEAD; ++k) {
+          raw[k] = raw[k + 1];
+          whole[k] = whole[k + 1];
+        }
+      }
     }
   }
 
@@ -477,34 +512,19 @@ struct Row {
       else s.list[at] = entry;
     }
   }
-  // f(values, row index of the first), by whole warps
-  template <typename F>
-  __device__ __forceinline__ void each_warp(F &&f) {
-    for (int vb = v0; vb < v1; vb += 32) {
-      const int vv = vb + lane;
-      float x[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = -INFINITY;
-      int at = 0;
-      if (vv < v1) at = vector(vv, x);
-      f(x, at);
-    }
-  }
   // Appends the elements in bins [lo, hi] that the cut keeps.
   __device__ __forceinline__ void append(const Cut &c, int lo, int hi, const float (&x)[E], int i0) {
-    float top = x[0], low = x[0];
-#pragma unroll
-    for (int e = 1; e < E; ++e) {
-      top = fmaxf(top, x[e]);
-      low = fminf(low, x[e]);
-    }
-    // most vectors hold none
-    if (!__any_sync(0xffffffffu, top > -INFINITY && bin_of(top) <= hi && (lo <= 0 || bin_of(low) >= lo))) return;
+    const float from = (float)lo, to = hi >= NB - 1 ? INFINITY : (float)(hi + 1);
+    bool take[E], any = false;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int b = x[e] > -INFINITY ? bin_of(x[e]) : NB;
-      append(b >= lo && b <= hi && kept(c, x[e], i0 + e), x[e], i0 + e);
+      const float d = depth(x[e]);
+      take[e] = d >= from && d < to && x[e] > -INFINITY;
+      any = any || take[e];
     }
+    if (!__any_sync(0xffffffffu, any)) return;       // most vectors hold none
+#pragma unroll
+    for (int e = 0; e < E; ++e) append(take[e] && kept(c, x[e], i0 + e), x[e], i0 + e);
   }
   // Descending bitonic sort of the list (all threads of CTA 0).
   __device__ void sort(u64 *a, int n) {
@@ -528,21 +548,19 @@ struct Row {
       }
     __syncthreads();
   }
-  // s.mass[i] <- sum of the weights of list entries 0 .. i (CTA 0).  Fixed order: eight consecutive entries a thread.
+  // s.mass[i] <- sum of the weights of list entries 0 .. i (CTA 0).  Fixed order: consecutive entries a thread.
   __device__ void accumulate(int n) {
-    constexpr int PER = CAP / THREADS;
-    double w[PER], sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = threadIdx.x * PER + i;
-      w[i] = e < n ? weight(value_of((uint32_t)(s.list[e] >> 32))) : 0.0;
-      sum += w[i];
+    const int per = (n + THREADS - 1) / THREADS, e0 = min((int)threadIdx.x * per, n), e1 = min(e0 + per, n);
+    double sum = 0.0;
+    for (int e = e0; e < e1; ++e) {
+      const double w = weight(value_of((uint32_t)(s.list[e] >> 32)));
+      s.mass[e] = w;
+      sum += w;
     }
     double run = exclusive<double>(sum, s.warp_sum);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      run += w[i];
-      s.mass[threadIdx.x * PER + i] = run;
+    for (int e = e0; e < e1; ++e) {
+      run += s.mass[e];
+      s.mass[e] = run;
     }
     __syncthreads();
   }
@@ -583,7 +601,7 @@ struct Row {
     double sum = 0.0, cta[C];
     const bool total_needed = top_p < 1.0f && top_k <= 0;
     const Cut all = {kNoCut, 0x7fffffff};
-    each_warp([&](const float (&x)[E], int i) {
+    each([&](const float (&x)[E], int i) {
       append(all, 0, last, x, i);
       if (total_needed) {
         double w[E];
@@ -646,7 +664,7 @@ struct Row {
     const int rank_in = top_k - (int)s.before_k;     // 1 ..
     list_reset();
     const Cut all = {kNoCut, 0x7fffffff};
-    each_warp([&](const float (&x)[E], int i) { append(all, b, b, x, i); });
+    each([&](const float (&x)[E], int i) { append(all, b, b, x, i); });
     cluster_barrier();
     if (rank == 0) {
       const int n = (int)min(s.n, (uint32_t)CAP);
@@ -665,14 +683,14 @@ struct Row {
     const int lo = s.b_p - 1, hi = s.b_p + 1;
     list_reset();
     double sum = 0.0, above = 0.0, cta[C];
-    each_warp([&](const float (&x)[E], int i) {
+    each([&](const float (&x)[E], int i) {
       append(cut, lo, hi, x, i);
       double w[E];
       weigh(cut, x, i, w);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         sum += w[e];
-        above += x[e] > -INFINITY && bin_of(x[e]) < lo ? w[e] : 0.0;
+        if (depth(x[e]) < (float)lo) above += w[e];   // (-inf weighs 0)
       }
     });
     const double total = cluster_total(sum, cta);
