@@ -33,8 +33,9 @@ typedef unsigned long long u64;
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int NB = 2048;           // histogram bins
 constexpr int CAP = 4096;          // list entries
+constexpr int SHORT = 1024;        // of a list that is ranked by counting, and in which all the rest may happen
 constexpr int MAXC = 8;
-constexpr int kLevelBits = 7, kLevels = 1 << kLevelBits;  // of the exponential's table
+constexpr int kLevelBits = 10, kLevels = 1 << kLevelBits;  // of the exponential's table
 constexpr uint32_t kNoCut = 0x007fffffu;  // key of -inf
 
 struct Params {
@@ -65,7 +66,7 @@ struct Cut {
 
 struct Shared {
   uint32_t count[NB];
-  u64 list[CAP];               // (key, ~index); the key histograms' two mass words lie here too
+  alignas(16) u64 list[CAP];               // (key, ~index); the key histograms' two mass words lie here too
   double mass[CAP];                 // of the sorted list: weights, then running sums
   double table[kLevels];            // 2^(-i / kLevels)
   double warp_sum[WARPS];
@@ -116,7 +117,7 @@ struct Row {
   int v0, v1;             // this warp's contiguous part of the slice, in 16-byte vectors from that boundary
   int first;              // row index of slice element 0
   float m, f_bin;         // maximum; bins per unit of value
-  double scale, offset;   // (x, T) -> kLevels * log2 of the weight
+  double top, scale;      // the maximum; kLevels * log2(e) / T
   float scale32, v_min;
   bool infinite;          // the maximum is: the elements come as the largest finite value, or as -inf
   int flip;
@@ -132,18 +133,18 @@ struct Row {
     return C > 1 ? tc::map_to_rank(l, (uint32_t)r) : l;
   }
   // exp((v - m) / T) in 64 bits: y = kLevels * log2(e) * (v - m) / T = k + f, |f| <= 1/2; 2^(k / kLevels) from the table and the
-  // exponent, 2^(f / kLevels) by its Taylor series (degree 3: the next term is below 0.0028^4 / 24 = 3e-12, two
-  // orders under what the sums need).  Below v_min the weight, 2^-1000, counts as 0.
+  // exponent, 2^(f / kLevels) by its Taylor series (degree 2: the next term is below 0.00034^3 / 6 = 7e-12, an order
+  // under what the sums need).  Below v_min the weight, 2^-1000, counts as 0.
   __device__ __forceinline__ double weight(float v) const { return v < v_min ? 0.0 : weight_above(v); }
   __device__ __forceinline__ double weight_above(float v) const {   // v >= v_min
-    const double y = fma((double)v, scale, offset);
+    // the difference first: it is exact where it counts, however large the logits are
+    const double d = (double)v - top;
     const double magic = 6755399441055744.0;         // 1.5 * 2^52: the sum's low word is the rounded y
-    const double z = y + magic;
+    const double z = fma(d, scale, magic);
     const int k = -__double2loint(z);
-    const double f = y - (z - magic);
+    const double f = fma(d, scale, magic - z);
     constexpr double L = 0.693147180559945309417 / kLevels;
-    double r = fma(L * L * L / 6.0, f, L * L / 2.0);
-    r = fma(r, f, L);
+    double r = fma(L * L / 2.0, f, L);
     r = fma(r, f, 1.0);
     const double w = r * s.table[k & (kLevels - 1)];
     return __hiloint2double(__double2hiint(w) - ((k & ~(kLevels - 1)) << (20 - kLevelBits)), __double2loint(w));
@@ -169,6 +170,31 @@ struct Row {
 #pragma unroll
       for (int e = 0; e < E; ++e)
         if (x[e] == at && i0 + e > c.index) w[e] = 0.0;
+    }
+  }
+  // sum += their sum; and, of those less deep than `upper` bins, above += it.
+  template <bool ABOVE>
+  __device__ __forceinline__ void add_weights(const Cut &c, const float (&x)[E], int i0, double &sum, float upper, double &above) const {
+    const float at = value_of(c.key), low = fmaxf(at, v_min);
+    float top = x[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
+    if (top < low) return;
+    if (i0 + E - 1 > c.index) {
+      double w[E];
+      weigh(c, x, i0, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        sum += w[e];
+        if (ABOVE && depth(x[e]) < upper) above += w[e];
+      }
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const double w = weight_above(x[e]);
+      if (x[e] >= low) sum += w;
+      if (ABOVE && x[e] >= low && depth(x[e]) < upper) above += w;
     }
   }
   // Lowest key whose weight is at least min_p: weights do not fall as keys rise.
@@ -275,17 +301,17 @@ struct Row {
     return total;
   }
 
-  // Lowest row index at which the inclusive sum of f exceeds target(total); -1 if the sum is empty.  The warp that
-  // finds it returns it, all others -1.
-  template <typename F, typename G>
-  __device__ int ordered_find(F &&f, G &&target) {
+  // Lowest row index at which the inclusive sum of a weighting exceeds target(total); -1 if the sum is empty.  The warp that
+  // finds it returns it, all others -1.  f(x, i, w) weighs a vector, g(x, i, sum) adds its weights up.
+  template <typename F, typename S, typename G>
+  __device__ int ordered_find(F &&f, S &&g, G &&target) {
     double v = 0.0;
-    each([&](const float (&x)[E], int i) {
-      double w[E];
-      f(x, i, w);
-#pragma unroll
-      for (int e = 0; e < E; ++e) v += w[e];
-    });
+    each([&](const float (&x)[E], int i) { g(x, i, v); });
+    return place(v, f, target);
+  }
+  // The same from the sums of the lanes of this warp.
+  template <typename F, typename G>
+  __device__ int place(double v, F &&f, G &&target) {
     double cta[C];
     const double total = cluster_total(v, cta);
     if (!(total > 0.0)) return -1;
@@ -526,8 +552,32 @@ struct Row {
 #pragma unroll
     for (int e = 0; e < E; ++e) append(take[e] && kept(c, x[e], i0 + e), x[e], i0 + e);
   }
-  // Descending bitonic sort of the list (all threads of CTA 0).
+  // Sorts the list, descending (all threads of CTA 0).  Entries differ, so a short list is ranked by counting the larger
+  // ones (64 to 1024 entries: 1 to 9 thousand cycles; the bitonic network takes 6 to 20, its steps are all latency).
   __device__ void sort(u64 *a, int n) {
+    if (n <= SHORT) {
+      constexpr int PER = SHORT / THREADS;
+      u64 mine[PER];
+      int rank_of[PER];
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        mine[k] = threadIdx.x + k * THREADS < n ? a[threadIdx.x + k * THREADS] : 0;
+        rank_of[k] = 0;
+      }
+      if (threadIdx.x == 0 && (n & 1)) a[n] = 0;
+      __syncthreads();
+      for (int i = 0; i < n; i += 2) {
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(a + i);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) rank_of[k] += (q.x > mine[k]) + (q.y > mine[k]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (threadIdx.x + k * THREADS < n) a[rank_of[k]] = mine[k];
+      __syncthreads();
+      return;
+    }
     int size = 2;
     while (size < n) size *= 2;
     for (int i = n + threadIdx.x; i < size; i += THREADS) a[i] = 0;
@@ -603,12 +653,8 @@ struct Row {
     const Cut all = {kNoCut, 0x7fffffff};
     each([&](const float (&x)[E], int i) {
       append(all, 0, last, x, i);
-      if (total_needed) {
-        double w[E];
-        weigh(all, x, i, w);
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum += w[e];
-      }
+      double none;
+      if (total_needed) add_weights<false>(all, x, i, sum, 0.f, none);
     });
     double total = 0.0;
     if (total_needed) total = cluster_total(sum, cta);
@@ -679,19 +725,15 @@ struct Row {
     return broadcast(cut);
   }
   // p of the mass: guessed to lie in bin b_p or beside it.
-  __device__ bool refine_p(Cut &cut, float top_p) {
+  // With one CTA a row it also leaves what draw_above needs: `above`, this lane's sum over the bins before those.
+  __device__ bool refine_p(Cut &cut, float top_p, double &above) {
     const int lo = s.b_p - 1, hi = s.b_p + 1;
     list_reset();
-    double sum = 0.0, above = 0.0, cta[C];
+    double sum = 0.0, cta[C];
+    above = 0.0;
     each([&](const float (&x)[E], int i) {
       append(cut, lo, hi, x, i);
-      double w[E];
-      weigh(cut, x, i, w);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        sum += w[e];
-        if (depth(x[e]) < (float)lo) above += w[e];   // (-inf weighs 0)
-      }
+      add_weights<true>(cut, x, i, sum, (float)lo, above);
     });
     const double total = cluster_total(sum, cta);
     const double over = cluster_total(above, cta);
@@ -706,6 +748,7 @@ struct Row {
         const int fits = prefix_length(n, [&](int i) { return over + (i ? s.mass[i - 1] : 0.0) < need; });
         ok = (fits > 0 || lo <= 0) && (fits < n || over + s.mass[n - 1] >= need || hi >= NB - 1);
         const int at = max(fits, 1) - 1;
+        if (threadIdx.x == 0) s.n = (uint32_t)at + 1;   // the entries that stay
         if (threadIdx.x == 0) s.cut = {(uint32_t)(s.list[at] >> 32), (int)~(uint32_t)s.list[at]};
       }
       __syncthreads();
@@ -713,6 +756,18 @@ struct Row {
       __syncthreads();
     }
     return broadcast(cut);
+  }
+
+  // The draw after refine_p, without another pass over the row: a warp's kept mass is what lies above the list's bins
+  // and the list entries of its part that stay.
+  __device__ int draw_above(const Cut &cut, double above, float u) {
+    const int keep = (int)s.n;
+    for (int i = lane; i < keep; i += 32) {
+      const int v = ((int)~(uint32_t)s.list[i] - first + shift) / E;
+      if (v >= v0 && v < v1) above += weight(value_of((uint32_t)(s.list[i] >> 32)));
+    }
+    return place(above, [&](const float (&x)[E], int i, double (&w)[E]) { weigh(cut, x, i, w); },
+                 [&](double total) { return (double)u * total; });
   }
 
   // ------------------------------------------------------------ a cut by histograms alone
@@ -823,6 +878,10 @@ struct Row {
         [&](const float (&x)[E], int j, double (&w)[E]) {
 #pragma unroll
           for (int e = 0; e < E; ++e) w[e] = key_of(x[e]) == k && kept(in, x[e], j + e) ? 1.0 : 0.0;
+        },
+        [&](const float (&x)[E], int j, double &sum) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) sum += key_of(x[e]) == k && kept(in, x[e], j + e) ? 1.0 : 0.0;
         },
                                [&](double) { return t - 0.5; });
     if (i >= 0 && lane == 0)
@@ -947,21 +1006,21 @@ sample_kernel(const Params p) {
     r.m = value_of((uint32_t)(best >> 32));
     const double c = 1.4426950408889634074 / (double)T0;
     r.scale = c * kLevels;
-    r.offset = -(double)r.m * r.scale;
+    r.top = (double)r.m;
     r.scale32 = (float)c;
     if (top_k >= p.V) top_k = 0;
     r.v_min = (float)((double)r.m - 1000.0 / c);
     if (r.m == INFINITY) {        // weight 1 for its like, 0 for any other: as if both were the largest finite value
       r.infinite = true;
       r.m = 3.402823466e38f;
-      r.scale = r.offset = 0.0;
+      r.top = (double)r.m;
       r.v_min = r.m;
     }
     Cut cut = {kNoCut, 0x7fffffff};
     bool drawn = false;
     if (top_k > 0 || top_p < 1.0f) {
       r.plan(cut, top_k, top_p, min_p, mn);
-      if (s.n_last <= CAP) {
+      if (s.n_last <= SHORT) {
         token = r.from_list(top_k, top_p, min_p, u);
         drawn = token != -2;
         if (!drawn) token = -1;
@@ -969,13 +1028,18 @@ sample_kernel(const Params p) {
       if (!drawn) {
         const int n_p = s.n_guess - s.n_first;   // logits around the guess
         if (top_k > 0 && !r.refine_k(cut, top_k)) cut = r.template descend<false>(cut, (double)top_k, 0.0);
-        if (top_p < 1.0f && !(n_p <= CAP && r.refine_p(cut, top_p))) {
+        double above = 0.0;
+        const bool refined = top_p < 1.0f && n_p <= CAP && r.refine_p(cut, top_p, above);
+        if (refined && C == 1 && (min_p <= 0.0f || r.min_p_key(min_p) <= cut.key)) {
+          token = r.draw_above(cut, above, u);
+          if (r.lane) token = -1;
+          drawn = true;
+        }
+        if (top_p < 1.0f && !refined) {
           double part = 0.0, cta[C];
           r.each([&](const float (&x)[E], int i) {
-            double w[E];
-            r.weigh(cut, x, i, w);
-#pragma unroll
-            for (int e = 0; e < E; ++e) part += w[e];
+            double none;
+            r.template add_weights<false>(cut, x, i, part, 0.f, none);
           });
           const double units = 17592186044416.0 / r.cluster_total(part, cta);  // 2^44 in all
           cut = r.template descend<true>(cut, fmax((double)top_p * 17592186044416.0, 1.0), units);
@@ -988,6 +1052,10 @@ sample_kernel(const Params p) {
         if (k > cut.key) cut = {k, 0x7fffffff};
       }
       token = r.ordered_find([&](const float (&x)[E], int i, double (&w)[E]) { r.weigh(cut, x, i, w); },
+                             [&](const float (&x)[E], int i, double &sum) {
+                               double none;
+                               r.template add_weights<false>(cut, x, i, sum, 0.f, none);
+                             },
                              [&](double total) { return (double)u * total; });
       if (r.lane) token = -1;
     }
