@@ -549,11 +549,31 @@ def rope(x, out, theta: float = 10000.0) -> None:
         out.copy_(od)
 
 
-def _lead(t: torch.Tensor, what: str):
+# ---- serving operators.  A decode step makes several of these calls per layer on a few rows each, where the time of a call
+# is the host's: their checks read each tensor's shape, strides and device once.
+_I64x8, _I64x10 = C.c_int64 * 8, C.c_int64 * 10
+
+
+def _on_host(*ts) -> bool:
+    for t in ts:
+        if t is not None and not t.is_cuda:
+            return True
+    return False
+
+
+def _one_device(what: str, first, *ts):
+    idx = first.get_device()
+    for t in ts:
+        if t is not None and t.get_device() != idx:
+            raise ValueError(f"{what}: all tensors of one call must live on the same device")
+    return first.device
+
+
+def _lead(what: str, shape, stride):
     """Strides of all but the last dimension (which must be 1); a dimension of one element counts as 0."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if shape[-1] > 1 and stride[-1] != 1:
         raise ValueError(f"{what}: innermost stride must be 1")
-    return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(t.dim() - 1)]
+    return [st if n > 1 else 0 for n, st in zip(shape[:-1], stride)]
 
 
 def _rotary(what: str, D: int, rotary_dim, theta: float, positions, tokens: int) -> int:
@@ -570,8 +590,8 @@ def _rotary(what: str, D: int, rotary_dim, theta: float, positions, tokens: int)
     return rot
 
 
-def _gain(what: str, w, D: int, like: torch.Tensor):
-    if w is not None and (w.shape != (D,) or w.dtype != like.dtype or not w.is_contiguous()):
+def _gain(what: str, w, D: int, dtype):
+    if w is not None and (w.dtype != dtype or w.shape != (D,) or not w.is_contiguous()):
         raise ValueError(f"{what}: a norm weight must be a contiguous [D] vector of the tensors' dtype")
 
 
@@ -587,26 +607,28 @@ def qk_norm_rope(q, k, q_out, k_out, positions=None, q_weight=None, k_weight=Non
     Weights None: ones.  Composed from rms_norm_fwd_kernel (test/python/triton/test_rms_norm.py:37-63) and
     rope_kernel (test/python/triton/test_rope.py:98-190)."""
     lib = _lib.load()
-    if any(t is not None and t.device.type != "cuda" for t in (q, k, q_out, k_out, positions, q_weight, k_weight)):
+    if _on_host(q, k, q_out, k_out, positions, q_weight, k_weight):
         return _stage(lambda q, k, q_out, k_out, positions, q_weight, k_weight: qk_norm_rope(
             q, k, q_out, k_out, positions, q_weight, k_weight, eps, theta, rotary_dim, interleaved),
             dict(q=q, k=k, q_out=q_out, k_out=k_out, positions=positions, q_weight=q_weight, k_weight=k_weight),
             ("q_out", "k_out"))
-    dev = _same_place(q, k, q_out, k_out, positions, q_weight, k_weight)
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+    dev = _one_device("qk_norm_rope", q, k, q_out, k_out, positions, q_weight, k_weight)
+    qs, ks, dtype = q.shape, k.shape, q.dtype
+    if len(qs) != 3 or len(ks) != 3 or qs[0] != ks[0] or qs[2] != ks[2]:
         raise ValueError("qk_norm_rope: expected q [tokens, q_heads, D] and k [tokens, kv_heads, D]")
-    if q_out.shape != q.shape or k_out.shape != k.shape or not (q.dtype == k.dtype == q_out.dtype == k_out.dtype):
+    if q_out.shape != qs or k_out.shape != ks or not (dtype == k.dtype == q_out.dtype == k_out.dtype):
         raise ValueError("qk_norm_rope: outputs must have the inputs' shapes and dtype")
     dt = _dt(q)
-    T, Hq, D = q.shape
+    T, Hq, D = qs
     rot = _rotary("qk_norm_rope", D, rotary_dim, theta, positions, T)
-    _gain("qk_norm_rope", q_weight, D, q)
-    _gain("qk_norm_rope", k_weight, D, k)
-    st = (C.c_int64 * 8)(*_lead(q, "q"), *_lead(k, "k"), *_lead(q_out, "q_out"), *_lead(k_out, "k_out"))
+    _gain("qk_norm_rope", q_weight, D, dtype)
+    _gain("qk_norm_rope", k_weight, D, dtype)
+    st = _I64x8(*_lead("q", qs, q.stride()), *_lead("k", ks, k.stride()), *_lead("q_out", qs, q_out.stride()),
+                *_lead("k_out", ks, k_out.stride()))
     with _guard(dev):
-        check(lib.hexb_qk_norm_rope(dt, _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), _ptr(positions), _ptr(q_weight),
-                                    _ptr(k_weight), T, Hq, k.shape[1], D, st, rot, int(bool(interleaved)), float(theta),
-                                    float(eps), _stream(q)), "qk_norm_rope")
+        check(lib.hexb_qk_norm_rope(dt, q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), _ptr(positions),
+                                    _ptr(q_weight), _ptr(k_weight), T, Hq, ks[1], D, st, rot, 1 if interleaved else 0,
+                                    theta, eps, _stream(q)), "qk_norm_rope")
 
 
 def kv_cache_append(k, v, k_cache, v_cache, slots, positions=None, k_weight=None, k_norm=None, eps: float = 1e-6,
@@ -622,41 +644,49 @@ def kv_cache_append(k, v, k_cache, v_cache, slots, positions=None, k_weight=None
     ``check_slots=True`` validates the slots first -- one device synchronisation -- and raises IndexError for
     one outside the cache, ValueError for one that is named twice."""
     lib = _lib.load()
-    if any(t is not None and t.device.type != "cuda" for t in (k, v, k_cache, v_cache, slots, positions, k_weight)):
+    if _on_host(k, v, k_cache, v_cache, slots, positions, k_weight):
         return _stage(lambda k, v, k_cache, v_cache, slots, positions, k_weight: kv_cache_append(
             k, v, k_cache, v_cache, slots, positions, k_weight, k_norm, eps, theta, rotary_dim, interleaved, check_slots),
             dict(k=k, v=v, k_cache=k_cache, v_cache=v_cache, slots=slots, positions=positions, k_weight=k_weight),
             ("k_cache", "v_cache"))
-    dev = _same_place(k, v, k_cache, v_cache, slots, positions, k_weight)
-    if k.dim() != 3 or k.shape != v.shape:
+    dev = _one_device("kv_cache_append", k, v, k_cache, v_cache, slots, positions, k_weight)
+    ks, cs, dtype = k.shape, k_cache.shape, k.dtype
+    if len(ks) != 3 or v.shape != ks:
         raise ValueError("kv_cache_append: expected k and v of one shape [tokens, kv_heads, D]")
-    T, H, D = k.shape
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or tuple(k_cache.shape[2:]) != (H, D):
+    T, H, D = ks
+    if len(cs) != 4 or v_cache.shape != cs or cs[2] != H or cs[3] != D:
         raise ValueError("kv_cache_append: expected caches of one shape [num_pages, page_size, kv_heads, D]")
-    if not (k.dtype == v.dtype == k_cache.dtype == v_cache.dtype):
+    if not (dtype == v.dtype == k_cache.dtype == v_cache.dtype):
         raise TypeError("kv_cache_append: k, v and the caches must share a dtype")
     dt = _dt(k)
     if slots.dtype != torch.int64 or slots.shape != (T,) or not slots.is_contiguous():
         raise ValueError("kv_cache_append: slots must be a contiguous int64 [tokens] vector")
     rot = _rotary("kv_cache_append", D, rotary_dim, theta, positions, T)
-    _gain("kv_cache_append", k_weight, D, k)
-    pages, page_size = k_cache.shape[:2]
+    _gain("kv_cache_append", k_weight, D, dtype)
+    pages, page_size = cs[0], cs[1]
     if T and page_size < 1:
         raise ValueError("kv_cache_append: the pages hold no slot")
+    norm = k_weight is not None if k_norm is None else bool(k_norm)
+    if k_weight is not None and not norm:
+        raise ValueError("kv_cache_append: a k_weight without the norm it belongs to")
     if check_slots and T:
         used = slots[slots >= 0]
         if used.numel() and int(used.max()) >= pages * page_size:
             raise IndexError(f"kv_cache_append: slot {int(used.max())} is outside the cache of {pages * page_size}")
         if used.unique().numel() != used.numel():
             raise ValueError("kv_cache_append: a slot is named twice")
-    st = (C.c_int64 * 10)(*_lead(k, "k"), *_lead(v, "v"), *_lead(k_cache, "k_cache"), *_lead(v_cache, "v_cache"))
-    norm = k_weight is not None if k_norm is None else bool(k_norm)
-    if k_weight is not None and not norm:
-        raise ValueError("kv_cache_append: a k_weight without the norm it belongs to")
+    st = _I64x10(*_lead("k", ks, k.stride()), *_lead("v", ks, v.stride()), *_lead("k_cache", cs, k_cache.stride()),
+                 *_lead("v_cache", cs, v_cache.stride()))
     with _guard(dev):
-        check(lib.hexb_kv_cache_append(dt, _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(slots),
-                                       _ptr(positions), _ptr(k_weight), T, H, D, pages, page_size, st, int(norm), rot,
-                                       int(bool(interleaved)), float(theta), float(eps), _stream(k)), "kv_cache_append")
+        check(lib.hexb_kv_cache_append(dt, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                       slots.data_ptr(), _ptr(positions), _ptr(k_weight), T, H, D, pages, page_size, st,
+                                       1 if norm else 0, rot, 1 if interleaved else 0, theta, eps, _stream(k)),
+              "kv_cache_append")
+
+
+def _indexes(name: str, t, dim: int):
+    if t is not None and (t.dtype != torch.int32 or t.dim() != dim or (t.stride(-1) != 1 and t.shape[-1] > 1)):
+        raise ValueError(f"shared_prefix_attention: {name} must be int32 with {dim} dimension(s) and unit stride")
 
 
 def shared_prefix_attention(q, k_cache, v_cache, out, prefix_pages=None, prefix_len: int = 0, block_table=None,
@@ -670,56 +700,56 @@ def shared_prefix_attention(q, k_cache, v_cache, out, prefix_pages=None, prefix_
     its new tokens: token i of nq sees the prefix_len prefix keys and its own keys j <= seq_lens[b] - nq + i.  Own
     key j is slot j % page_size of page block_table[b, j // page_size] (int32 [batch, width]); prefix keys lie in
     prefix_pages (int32) the same way.  A token that sees no key gets zeros; rows from q_offsets[-1] on are left as
-    they are.  max_q: the usual number of new tokens of a sequence -- it shapes the launch, any value is right.
+    they are.  Values that some new token of a sequence sees and another does not must be finite.  max_q: the
+    usual number of new tokens of a sequence -- it shapes the launch, any value is right.
 
     Lengths, tables and offsets stay on the device and are read by every launch, so a captured CUDA graph
     follows them; only prefix_len and the shapes are fixed at capture.  A page outside the cache reads as zeros, a
     length beyond the table is cut; both record HEXB_ERR_BAD_ARG in the device status word.
     The softmax and its scale are those of ``attention`` (test/python/triton/test_flash_attention.py:37-168)."""
     lib = _lib.load()
-    every = dict(q=q, k_cache=k_cache, v_cache=v_cache, out=out, prefix_pages=prefix_pages, block_table=block_table,
-                 seq_lens=seq_lens, q_offsets=q_offsets)
-    if any(t is not None and t.device.type != "cuda" for t in every.values()):
+    if _on_host(q, k_cache, v_cache, out, prefix_pages, block_table, seq_lens, q_offsets):
         return _stage(lambda q, k_cache, v_cache, out, prefix_pages, block_table, seq_lens, q_offsets:
                       shared_prefix_attention(q, k_cache, v_cache, out, prefix_pages, prefix_len, block_table, seq_lens,
-                                              q_offsets, max_q, sm_scale), every, ("out",))
-    dev = _same_place(*every.values())
-    if q.dim() != 3 or out.shape != q.shape:
+                                              q_offsets, max_q, sm_scale),
+                      dict(q=q, k_cache=k_cache, v_cache=v_cache, out=out, prefix_pages=prefix_pages,
+                           block_table=block_table, seq_lens=seq_lens, q_offsets=q_offsets), ("out",))
+    dev = _one_device("shared_prefix_attention", q, k_cache, v_cache, out, prefix_pages, block_table, seq_lens, q_offsets)
+    qs, cs = q.shape, k_cache.shape
+    if len(qs) != 3 or out.shape != qs:
         raise ValueError("shared_prefix_attention: expected q and out of one shape [tokens, q_heads, D]")
-    T, Hq, D = q.shape
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != D:
+    T, Hq, D = qs
+    if len(cs) != 4 or v_cache.shape != cs or cs[3] != D:
         raise ValueError("shared_prefix_attention: expected caches of one shape [num_pages, page_size, kv_heads, D]")
     if not (q.dtype == out.dtype == k_cache.dtype == v_cache.dtype == torch.float16):
         raise TypeError("shared_prefix_attention: float16 tensors expected")
-    pages, page_size, Hkv, _ = k_cache.shape
+    pages, page_size, Hkv, _ = cs
     if Hkv == 0 or Hq % Hkv or page_size < 1:
         raise ValueError("shared_prefix_attention: q_heads must be a multiple of kv_heads, page_size positive")
-    for name, t, dim in (("prefix_pages", prefix_pages, 1), ("block_table", block_table, 2), ("seq_lens", seq_lens, 1),
-                         ("q_offsets", q_offsets, 1)):
-        if t is not None and (t.dtype != torch.int32 or t.dim() != dim or (t.numel() > 1 and t.stride(-1) != 1)):
-            raise ValueError(f"shared_prefix_attention: {name} must be int32 with {dim} dimension(s) and unit stride")
-    if prefix_len < 0 or max_q < 0 or (prefix_len and (prefix_pages is None or prefix_pages.numel() * page_size < prefix_len)):
+    _indexes("prefix_pages", prefix_pages, 1)
+    _indexes("block_table", block_table, 2)
+    _indexes("seq_lens", seq_lens, 1)
+    _indexes("q_offsets", q_offsets, 1)
+    if prefix_len < 0 or max_q < 0 or (prefix_len and (prefix_pages is None or prefix_pages.shape[0] * page_size < prefix_len)):
         raise ValueError("shared_prefix_attention: prefix_pages do not hold prefix_len keys")
     if (block_table is None) != (seq_lens is None):
         raise ValueError("shared_prefix_attention: block_table and seq_lens belong together")
-    B = q_offsets.numel() - 1 if q_offsets is not None else T
-    if B < 0 or (block_table is not None and (block_table.shape[0] != B or seq_lens.numel() != B)):
+    B = q_offsets.shape[0] - 1 if q_offsets is not None else T
+    if B < 0 or (block_table is not None and (block_table.shape[0] != B or seq_lens.shape[0] != B)):
         raise ValueError("shared_prefix_attention: block_table, seq_lens and q_offsets disagree about the batch")
-    d = _lib.PagedAttentionDesc()
-    d.Q, d.K_cache, d.V_cache, d.Out = _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out)
-    d.prefix_pages, d.q_offsets = _ptr(prefix_pages), _ptr(q_offsets)
-    d.T, d.B, d.Hq, d.Hkv, d.D = T, B, Hq, Hkv, D
-    d.num_pages, d.page_size, d.prefix_len, d.max_q = pages, page_size, prefix_len, max_q
-    if block_table is not None:
-        d.block_table, d.seq_lens = _ptr(block_table), _ptr(seq_lens)
-        d.table_width, d.table_stride = block_table.shape[1], block_table.stride(0)
-    d.strides = (C.c_int64 * 10)(*_lead(q, "q"), *_lead(k_cache, "k_cache"), *_lead(v_cache, "v_cache"), *_lead(out, "out"))
-    d.sm_scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    width, row = (block_table.shape[1], block_table.stride(0)) if block_table is not None else (0, 0)
+    d = _lib.PagedAttentionDesc(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), _ptr(prefix_pages), _ptr(block_table),
+        _ptr(seq_lens), _ptr(q_offsets), T, B, Hq, Hkv, D, pages, page_size, prefix_len, width, row, max_q,
+        _I64x10(*_lead("q", qs, q.stride()), *_lead("k_cache", cs, k_cache.stride()),
+                *_lead("v_cache", cs, v_cache.stride()), *_lead("out", qs, out.stride())),
+        1.0 / math.sqrt(D) if sm_scale is None else sm_scale)
     with _guard(dev):
-        need = lib.hexb_paged_attention_workspace_bytes(C.byref(d))
+        ref = C.byref(d)
+        need = lib.hexb_paged_attention_workspace_bytes(ref)
         # from torch's allocator: its blocks follow the stream, and a captured graph keeps its own
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        check(lib.hexb_paged_attention_f16(C.byref(d), _ptr(ws), need, _stream(q)), "shared_prefix_attention")
+        check(lib.hexb_paged_attention_f16(ref, _ptr(ws), need, _stream(q)), "shared_prefix_attention")
 
 
 def sample_tokens(logits, u, out, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> None:
@@ -732,35 +762,31 @@ def sample_tokens(logits, u, out, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     index order, whose inclusive sum of w exceeds u times the kept sum.  temperature 0: the largest logit.
     Ties go to the lowest index.  NaN and -inf are never chosen; a row of nothing else gives -1."""
     lib = _lib.load()
-    tens = lambda v: v if torch.is_tensor(v) else None
-    every = dict(logits=logits, u=u, out=out, temperature=tens(temperature), top_k=tens(top_k), top_p=tens(top_p),
-                 min_p=tens(min_p))
-    if any(t is not None and t.device.type != "cuda" for t in every.values()):
+    tens = [v if isinstance(v, torch.Tensor) else None for v in (temperature, top_k, top_p, min_p)]
+    if _on_host(logits, u, out, *tens):
         pick = lambda a, b: b if a is None else a
-        return _stage(lambda logits, u, out, **k: sample_tokens(
-            logits, u, out, pick(k["temperature"], temperature), pick(k["top_k"], top_k), pick(k["top_p"], top_p),
-            pick(k["min_p"], min_p)), every, ("out",))
-    dev = _same_place(*every.values())
+        return _stage(lambda logits, u, out, t, k, p, m: sample_tokens(
+            logits, u, out, pick(t, temperature), pick(k, top_k), pick(p, top_p), pick(m, min_p)),
+            dict(logits=logits, u=u, out=out, t=tens[0], k=tens[1], p=tens[2], m=tens[3]), ("out",))
+    dev = _one_device("sample_tokens", logits, u, out, *tens)
     rows, vocab, xs = _rows2d(logits, "logits")
     dt = _dt(logits)
     if vocab < 1:
         raise ValueError("sample_tokens: no logits to choose from")
     if u.dtype != torch.float32 or out.dtype != torch.int64:
         raise TypeError("sample_tokens: u must be float32 and out int64")
-    for name, t, kind in (("u", u, u.dtype), ("out", out, out.dtype), ("temperature", every["temperature"], torch.float32),
-                          ("top_k", every["top_k"], torch.int32), ("top_p", every["top_p"], torch.float32),
-                          ("min_p", every["min_p"], torch.float32)):
-        if t is not None and (t.shape != (rows,) or t.dtype != kind or not t.is_contiguous()):
+    for name, t, kind in (("u", u, torch.float32), ("out", out, torch.int64), ("temperature", tens[0], torch.float32),
+                          ("top_k", tens[1], torch.int32), ("top_p", tens[2], torch.float32), ("min_p", tens[3], torch.float32)):
+        if t is not None and (t.dtype != kind or t.shape != (rows,) or not t.is_contiguous()):
             raise ValueError(f"sample_tokens: {name} must be a contiguous {kind} [rows] vector")
-    num = lambda name, v, off: off if every[name] is not None else v
-    t0, k0, p0, m0 = (num("temperature", temperature, 0.0), num("top_k", top_k, 0), num("top_p", top_p, 1.0),
-                      num("min_p", min_p, 0.0))
+    t0, k0, p0, m0 = (off if t is not None else v
+                      for t, v, off in zip(tens, (temperature, top_k, top_p, min_p), (0.0, 0, 1.0, 0.0)))
     if not (t0 >= 0 and k0 >= 0 and 0 <= p0 <= 1 and 0 <= m0 <= 1):
         raise ValueError("sample_tokens: temperature and top_k must not be negative, top_p and min_p lie in [0, 1]")
     with _guard(dev):
-        check(lib.hexb_sample_tokens(dt, _ptr(logits), _ptr(u), _ptr(out), rows, vocab, xs, _ptr(every["temperature"]),
-                                     _ptr(every["top_k"]), _ptr(every["top_p"]), _ptr(every["min_p"]), float(t0),
-                                     min(int(k0), 0x7fffffff), float(p0), float(m0), _stream(logits)), "sample_tokens")
+        check(lib.hexb_sample_tokens(dt, logits.data_ptr(), u.data_ptr(), out.data_ptr(), rows, vocab, xs, _ptr(tens[0]),
+                                     _ptr(tens[1]), _ptr(tens[2]), _ptr(tens[3]), t0, min(int(k0), 0x7fffffff), p0, m0,
+                                     _stream(logits)), "sample_tokens")
 
 
 class DecoderStack:

@@ -67,7 +67,7 @@ def meta(*shape, dtype=torch.float16):
     """A tensor that is refused before its data or device matter."""
     class Fake:
         def __init__(self, t):
-            self.t, self.device = t, torch.device("cuda:0")
+            self.t, self.device, self.is_cuda, self.get_device = t, torch.device("cuda:0"), True, lambda: 0
 
         def __getattr__(self, n):
             return getattr(self.t, n)
