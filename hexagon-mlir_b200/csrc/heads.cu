@@ -52,11 +52,11 @@ struct Params {
   uint64_t power[kPowerBits];
 };
 
-// Angles are fractions of a turn in 64-bit fixed point: 2^64 is one turn, a product with the position wraps as an
-// angle does, and no 64-bit floating-point chain delays the first row of a CTA (with one, a single token took
-// 6.0 us against 3.3).  The frequency of pair p is 2^64 / (2 pi) * theta^(-2p / rotary_dim): the product of the powers
-// theta^(-2^(b+1) / rotary_dim) over the bits b of p, which the host forms in 64-bit floating point (2^63 is 1):
-// relative error at most 12 * 2^-53, so the angle at position n is good to n * 2^-50 of a turn.
+// Angles are fractions of a turn in 64-bit fixed point: 2^64 is one turn, a product with the position wraps as an angle
+// does, and no chain of 64-bit floating-point operations delays the first row of a CTA.  The frequency of pair p is
+// 2^64 / (2 pi) * theta^(-2p / rotary_dim): the product of the powers theta^(-2^(b+1) / rotary_dim) over the bits b of p,
+// which the host forms in 64-bit floating point (2^63 is 1): relative error at most 12 * 2^-53, so the angle at position n
+// is good to n * 2^-50 of a turn.
 __device__ __forceinline__ uint64_t frequency(const Params &p, int pr) {
   uint64_t f = 2935890503282001226ull;  // 2^64 / (2 pi)
 #pragma unroll
@@ -102,8 +102,10 @@ __device__ __forceinline__ int64_t load_slot(const Params &p, int64_t token) {
 // once: the addresses advance by a constant, and the linear map of a row
 //   y_e = rstd * (A_e x_e + B_e x_partner(e)),   A = w cos,  B = -+ w_partner sin
 // sits in registers -- two fused operations an element besides the mean.  The first row is requested before the
-// angles are computed, and the next while one is worked on.  The code is kept to one copy of each step: with
-// few tokens the time is that of fetching it.
+// angles are computed, and the next while one is worked on.  8192 tokens of 16 + 4 heads of 128 (84 MB): 26 us, 3.2 TB/s;
+// append of 16400 tokens of 8 heads (134 MB): 37 us, 3.6 TB/s; one token: 4.3 us back to back.  What bounds it now is
+// the latency of the few CTAs that the registers of the map allow an SM (37 % of the issue slots, 25 % of the memory rate);
+// smaller register budgets spill (80 registers: 36 us).
 template <typename T, int LPR, int NV>
 __global__ void __launch_bounds__(THREADS, 5)
 head_rows_kernel(const Params p) {

@@ -444,7 +444,8 @@ struct Row {
   //         b_last         the last bin that the list needs, n_last logits up to it; guessed: b_p set it
   //         n_first, n_guess   logits before bin b_p - 1, and up to bin b_p + 1
   __device__ void plan(const Cut &in, int top_k, float top_p, float min_p, float lowest) {
-    const float range = fminf(m - lowest, 32.0f);
+    // (a sample that is all masked, or all the maximum, says nothing about the width)
+    const float range = lowest < m ? fminf(m - lowest, 32.0f) : 32.0f;
     f_bin = range > 1e-20f ? (float)NB / range : 0.0f;
     clear(false);
     each([&](const float (&x)[E], int) {
@@ -525,20 +526,7 @@ struct Row {
     if (threadIdx.x == 0) s.n = 0;
     cluster_barrier();
   }
-  // Appends (v, i) to the list of CTA 0 where `take`; the whole warp calls it.
-  __device__ __forceinline__ void append(bool take, float v, int i) {
-    const unsigned who = __ballot_sync(0xffffffffu, take);
-    if (!who) return;
-    uint32_t at = 0;
-    if (lane == __ffs(who) - 1) at = C > 1 ? add_cluster_u32(peer(&s.n, 0), __popc(who)) : atomicAdd(&s.n, (uint32_t)__popc(who));
-    at = __shfl_sync(0xffffffffu, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1u));
-    if (take && at < CAP) {
-      const u64 entry = (u64)key_of(v) << 32 | (uint32_t)~i;
-      if (C > 1) st_cluster_u64(peer(&s.list[at], 0), entry);
-      else s.list[at] = entry;
-    }
-  }
-  // Appends the elements in bins [lo, hi] that the cut keeps.
+  // Appends the elements in bins [lo, hi] that the cut keeps to the list of CTA 0; the whole warp calls it.
   __device__ __forceinline__ void append(const Cut &c, int lo, int hi, const float (&x)[E], int i0) {
     const float from = (float)lo, to = hi >= NB - 1 ? INFINITY : (float)(hi + 1);
     bool take[E], any = false;
@@ -549,32 +537,56 @@ struct Row {
       any = any || take[e];
     }
     if (!__any_sync(0xffffffffu, any)) return;       // most vectors hold none
+    // One reservation for the warp's vectors: with a cluster it is a trip to CTA 0 and back.
+    unsigned who[E];
+    int all = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) append(take[e] && kept(c, x[e], i0 + e), x[e], i0 + e);
+    for (int e = 0; e < E; ++e) {
+      who[e] = __ballot_sync(0xffffffffu, take[e] && kept(c, x[e], i0 + e));
+      all += __popc(who[e]);
+    }
+    if (all == 0) return;
+    uint32_t at = 0;
+    if (lane == 0) at = C > 1 ? add_cluster_u32(peer(&s.n, 0), (uint32_t)all) : atomicAdd(&s.n, (uint32_t)all);
+    at = __shfl_sync(0xffffffffu, at, 0);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint32_t mine = at + __popc(who[e] & ((1u << lane) - 1u));
+      if ((who[e] >> lane & 1u) && mine < CAP) {
+        const u64 entry = (u64)key_of(x[e]) << 32 | (uint32_t)~(i0 + e);
+        if (C > 1) st_cluster_u64(peer(&s.list[mine], 0), entry);
+        else s.list[mine] = entry;
+      }
+      at += __popc(who[e]);
+    }
   }
   // Sorts the list, descending (all threads of CTA 0).  Entries differ, so a short list is ranked by counting the larger
-  // ones (64 to 1024 entries: 1 to 9 thousand cycles; the bitonic network takes 6 to 20, its steps are all latency).
+  // ones (300 entries: 4 thousand cycles; the bitonic network takes 12, its steps are all latency).
   __device__ void sort(u64 *a, int n) {
     if (n <= SHORT) {
       constexpr int PER = SHORT / THREADS;
       u64 mine[PER];
-      int rank_of[PER];
+      int larger[PER];
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
         mine[k] = threadIdx.x + k * THREADS < n ? a[threadIdx.x + k * THREADS] : 0;
-        rank_of[k] = 0;
+        larger[k] = 0;
       }
       if (threadIdx.x == 0 && (n & 1)) a[n] = 0;
       __syncthreads();
-      for (int i = 0; i < n; i += 2) {
-        const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(a + i);
 #pragma unroll
-        for (int k = 0; k < PER; ++k) rank_of[k] += (q.x > mine[k]) + (q.y > mine[k]);
+      for (int k = 0; k < PER; ++k) {
+        if (warp * 32 + k * THREADS >= n) break;       // no entry in this warp
+#pragma unroll 4
+        for (int i = 0; i < n; i += 2) {
+          const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(a + i);
+          larger[k] += (q.x > mine[k]) + (q.y > mine[k]);
+        }
       }
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < PER; ++k)
-        if (threadIdx.x + k * THREADS < n) a[rank_of[k]] = mine[k];
+        if (threadIdx.x + k * THREADS < n) a[larger[k]] = mine[k];
       __syncthreads();
       return;
     }

@@ -54,7 +54,8 @@ def make(T, heads, D, dtype, seed):
 @pytest.mark.parametrize("interleaved", [True, False])
 @pytest.mark.parametrize("T,Hq,Hkv,D,rot", [
     (1, 16, 4, 128, 128), (3, 5, 1, 64, 64), (777, 12, 12, 64, 32), (65, 8, 2, 256, 256), (2049, 6, 2, 96, 96),
-    (33, 4, 4, 128, 0), (9, 3, 1, 80, 20), (7, 2, 1, 10, 6), (5, 1, 1, 2, 2), (4, 2, 1, 513, 512), (130, 40, 8, 128, 64)])
+    (33, 4, 4, 128, 0), (9, 3, 1, 80, 20), (7, 2, 1, 10, 6), (5, 1, 1, 2, 2), (4, 2, 1, 513, 512), (130, 40, 8, 128, 64), (70, 3, 2, 8, 8), (41, 2, 1, 16, 16), (12, 2, 2, 32, 32),
+    (6, 64, 8, 128, 128), (5, 2, 1, 1024, 1024), (2000, 1, 0, 64, 64), (300, 0, 3, 64, 64)])
 def test_qk_norm_rope_vs_formula(T, Hq, Hkv, D, rot, interleaved, dtype):
     q, k = make(T, Hq, D, dtype, 1), make(T, Hkv, D, dtype, 2)
     wq, wk = make(1, 1, D, dtype, 3).view(D), make(1, 1, D, dtype, 4).view(D)

@@ -109,6 +109,12 @@ CASES = [
     (12, 12, 64, 16, 64, [33, 64, 1], [40, 64, 500]),
     (16, 2, 128, 16, 4096, [1] * 40, [100] * 40),                 # many rows against a long prefix
     (24, 8, 128, 64, 777, [1] * 64, list(range(64))),             # three heads a group, many rows
+    (8, 2, 128, 8, 300, [1] * 40, [100] * 40),                    # the smallest page that TMA pieces fit
+    (8, 2, 64, 40, 300, [30, 41], [100, 90]),                     # pages of five pieces
+    (200, 1, 64, 16, 100, [1, 3], [30, 31]),                      # more heads a group than a tile has rows
+    (128, 1, 128, 16, 100, [2, 3], [30, 31]),
+    (2, 2, 128, 512, 700, [100, 90], [1500, 90]),                 # pages longer than a block
+    (6, 6, 64, 16, 90, [40], [40]),
     (2, 1, 128, 16, 20000, [1], [5]),
     (2, 1, 64, 16, 0, [1], [20000]),
 ]
@@ -146,6 +152,16 @@ def test_prefix_only(D, prefix, B, G):
     out = torch.empty_like(q)
     ops.shared_prefix_attention(q, kc, vc, out, prefix_pages, prefix)
     check(out, q, kc, vc, prefix_pages, prefix, None, [0] * B, [1] * B)
+
+
+@pytest.mark.parametrize("case", [0, 5, 11, 13, 16])
+def test_without_overlapping_launches(case):
+    """Option "pdl" 0: the launches of a call run one after the other."""
+    hexb200.set_option("pdl", 0)
+    try:
+        test_vs_softmax_in_64_bits(case, False)
+    finally:
+        hexb200.set_option("pdl", 1)
 
 
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])

@@ -146,6 +146,31 @@ def test_border_random_numbers_and_scalar_parameters():
     assert out.tolist()[:5] == [1, 2, 7, 7, 1]
 
 
+@pytest.mark.parametrize("rows", [2, 160])
+def test_rows_masked_but_for_few(rows):
+    """Constrained decoding: all but a few logits are -inf (or the lowest value), wherever they lie."""
+    V = 60000
+    g = torch.Generator().manual_seed(rows)
+    x = torch.full((rows, V), -float("inf"))
+    x[1::2] = torch.finfo(torch.float16).min
+    for r in range(rows):
+        at = torch.randperm(V, generator=g)[:100]
+        x[r, at] = torch.randn(100, generator=g) * 3
+    x = x.half().to(dev)
+    r = np.random.default_rng(4)
+    compare(x, r.random(rows, dtype=np.float32), r.choice([0.5, 1.0], rows), r.choice([0, 7, 200], rows),
+            r.choice([1.0, 0.9], rows), r.choice([0.0, 0.01], rows))
+
+
+@pytest.mark.parametrize("temp", [1e-40, 1e-3, 50.0, 1e30])
+def test_extreme_temperatures(temp):
+    """The definition's weights in 64 bits: near 0 the largest logits alone, far above 1 all alike."""
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(4, 30000, generator=g).to(dev)
+    x[1, 7] = x[1, 20000] = 9.0
+    compare(x, [0.1, 0.6, 0.5, 0.99], [temp] * 4, [0, 0, 500, 0], [1.0, 0.9, 0.9, 0.3], [0.0, 0.0, 0.0, 0.2])
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_strided_rows_of_any_alignment(dtype):
     g = torch.Generator().manual_seed(5)
