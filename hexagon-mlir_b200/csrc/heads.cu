@@ -27,6 +27,7 @@ static __device__ int g_heads_status = 0;
 namespace heads {
 
 constexpr int THREADS = 128;
+constexpr int AHEAD = 4;         // rows a group of lanes has under way
 constexpr int kPowerBits = 11;   // rotary_dim <= 4096
 
 // One of the two tensors a call walks (queries and keys, or keys and values).
@@ -67,6 +68,11 @@ __device__ __forceinline__ uint64_t frequency(const Params &p, int pr) {
   }
   return f;
 }
+__host__ __device__ constexpr int ring_bytes(int nv) { return AHEAD * nv * THREADS * 16; }
+__device__ __forceinline__ void copy16_async(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+
 // cos and sin of pos * frequency
 __device__ __forceinline__ float2 turn(int64_t pos, uint64_t freq) {
   const int32_t t = (int32_t)(((uint64_t)pos * freq) >> 32);
@@ -101,18 +107,19 @@ __device__ __forceinline__ int64_t load_slot(const Params &p, int64_t token) {
 // rotation formed anew for each: 80 us where the traffic takes 21), so what the rows of a group share is set up
 // once: the addresses advance by a constant, and the linear map of a row
 //   y_e = rstd * (A_e x_e + B_e x_partner(e)),   A = w cos,  B = -+ w_partner sin
-// sits in registers -- two fused operations an element besides the mean.  The first row is requested before the
-// angles are computed, and the next while one is worked on.  8192 tokens of 16 + 4 heads of 128 (84 MB): 26 us, 3.2 TB/s;
-// append of 16400 tokens of 8 heads (134 MB): 37 us, 3.6 TB/s; one token: 4.3 us back to back.  What bounds it now is
-// the latency of the few CTAs that the registers of the map allow an SM (37 % of the issue slots, 25 % of the memory rate);
-// smaller register budgets spill (80 registers: 36 us).
+// sits in registers -- two fused operations an element besides the mean.  AHEAD rows of a group are under way, the first
+// before the angles are computed.  The code is kept to one copy of each step: with few tokens the time is that of
+// fetching it.  8192 tokens of 16 + 4 heads of 128 (84 MB): 19 us, 4.4 TB/s; append of 16400 tokens of 8 heads (134 MB):
+// 30 us, 4.5 TB/s; one token: 4.3 us back to back.  Held in registers, one row ahead, they took 26 and 37 us: 20 KB
+// under way on an SM do not cover the latency of memory.  Four CTAs an SM without spills beat five with (22 against 25 us).
 template <typename T, int LPR, int NV>
-__global__ void __launch_bounds__(THREADS, 5)
+__global__ void __launch_bounds__(THREADS, 4)
 head_rows_kernel(const Params p) {
   constexpr int E = Vec16<T>::N;
   using Raw = decltype(Vec16<T>::raw);
   // cos, sin of pair (v, e) of vector v at [token][e][v]: the lanes of a row read consecutive words
-  extern __shared__ float2 s_cs[];
+  extern __shared__ __align__(16) uint8_t s_dyn[];
+  float2 *const s_cs = reinterpret_cast<float2 *>(s_dyn + ring_bytes(NV));
   const int lane = threadIdx.x % LPR, grp = threadIdx.x / LPR;
   const int nvec = p.D / E, half = p.rot / 2, rotv = p.rot / E, hv = half / E;
   const bool inter = p.interleaved != 0;
@@ -128,19 +135,21 @@ head_rows_kernel(const Params p) {
 
   const T *src = static_cast<const T *>(p.seg[0].src) + tok * p.seg[0].src_t + (int64_t)h0 * p.seg[0].src_h + lane * E;
   const T *src1 = static_cast<const T *>(p.seg[1].src) + tok * p.seg[1].src_t + (int64_t)h1 * p.seg[1].src_h + lane * E;
-  Raw raw[NV];
+  // Rows travel through shared memory, each lane's 16-byte pieces into places of its own: no barrier, and the rows under
+  // way cost no registers.
+  uint4 *const ring = reinterpret_cast<uint4 *>(s_dyn) + threadIdx.x;     // [AHEAD][NV][THREADS]
   auto request = [&](int n) {
     if (n < n0 + n1) {
       if (n == n0) src = src1;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        raw[i] = Raw{};
-        if (lane + i * LPR < nvec) raw[i] = ld_stream_as<Raw>(src + i * LPR * E);
-      }
+      for (int i = 0; i < NV; ++i)
+        if (lane + i * LPR < nvec) copy16_async(ring + ((n % AHEAD) * NV + i) * THREADS, src + i * LPR * E);
       src += p.seg[n >= n0].src_h << gs;
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  request(0);
+#pragma unroll
+  for (int n = 0; n < AHEAD; ++n) request(n);
   // the gains are needed after the angles: their fetch overlaps that of the positions (one token: 6.7 -> 6.2 us)
   if (threadIdx.x < 2 * LPR * NV) {
     const int g = threadIdx.x >= LPR * NV, v = threadIdx.x - g * LPR * NV;
@@ -168,6 +177,17 @@ head_rows_kernel(const Params p) {
   int64_t dst_step = 0;
 #pragma unroll 1
   for (int n = 0; n < n0 + n1; ++n) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+    Raw raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      raw[i] = Raw{};
+      if (lane + i * LPR < nvec) {
+        const uint4 v = ring[((n % AHEAD) * NV + i) * THREADS];
+        raw[i] = *reinterpret_cast<const Raw *>(&v);
+      }
+    }
+    request(n + AHEAD);
     if (n == 0 || n == n0) {
       const int g = n >= n0;
       const Segment &s = p.seg[g];
@@ -209,7 +229,6 @@ head_rows_kernel(const Params p) {
         for (int i = 0; i < NV; ++i)
           if (lane + i * LPR < nvec) st_stream_as<Raw>(dst + i * LPR * E, raw[i]);
       }
-      request(n + 1);
     } else {
       float f[NV][E], o[NV][E];
 #pragma unroll
@@ -248,7 +267,6 @@ head_rows_kernel(const Params p) {
           x.unpack(o[i]);
         }
       }
-      request(n + 1);
       float rstd = 1.0f;
       if (norm) {
         float ss = 0.f;
@@ -359,16 +377,17 @@ static int launch(Params p, float theta, cudaStream_t st) {
   const int nvec = p.D / E;
   const int lpr = nvec <= 8 ? 4 : nvec <= 16 ? 8 : nvec <= 32 ? 16 : 32;   // two vectors a lane
   const int rp = THREADS / lpr;
-  // Tokens per CTA: so many that a group of lanes gets four of a token's heads, but no fewer CTAs than two an SM.
+  // Tokens per CTA: so many that a group of lanes gets sixteen of a token's heads (the map is
+  // built for them once: with four, 27 us for the 8192 tokens), but no fewer CTAs than two an SM.
   int tb = 1;
-  while (tb < rp && rp / tb * 4 > p.seg[0].heads) tb *= 2;
+  while (tb < rp && rp / tb * 16 > p.seg[0].heads) tb *= 2;
   while (tb > 1 && (p.tokens + tb - 1) / tb < 2 * (int64_t)di.sm_count) tb /= 2;
   p.tokens_per_cta = tb;
   for (p.gpt_shift = 0; (tb << (p.gpt_shift + 1)) <= rp;) ++p.gpt_shift;
   const int64_t gx = (p.tokens + tb - 1) / tb;
   if (gx > 0x7fffffff) return HEXB_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)gx);
-  const size_t smem = (size_t)tb * (p.rot / 2) * sizeof(float2);
+  const size_t smem = ring_bytes(2) + (size_t)tb * (p.rot / 2) * sizeof(float2);
   cudaError_t e;
   if (lpr == 4) e = launch_vec<T, 4, 2>(p, grid, smem, st);
   else if (lpr == 8) e = launch_vec<T, 8, 2>(p, grid, smem, st);
