@@ -442,14 +442,21 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       const int cl = p.cluster, rank = (int)tc::cluster_ctarank();
       float2 *ml = reinterpret_cast<float2 *>(smem);                          // over Q: the last product has read it
       const uint32_t so = sK0;                                                // over K and V: [128 rows][HD], 16-byte pieces
+      float2 *fin = ml + 128;                                                 // of row r: maximum and sum over the cluster
       ml[r] = make_float2(m_last, l_last);                                    // of row r at (piece ^ r)
       tc::cluster_sync_all();
-      float mm = -INFINITY;
+      float mm = -INFINITY, ll = 0.f;
       const uint32_t mine = tc::smem_u32(&ml[r]);
-      for (int i = 0; i < cl; ++i) {
-        const float2 v = ld_cluster_f2(tc::map_to_rank(mine, (uint32_t)i));
-        if (v.y != 0.f) mm = fmaxf(mm, v.x);
-      }
+      float2 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)                                             // all trips to the peers under way at once
+        v[i] = i < cl ? ld_cluster_f2(tc::map_to_rank(mine, (uint32_t)i)) : make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (v[i].y != 0.f) mm = fmaxf(mm, v[i].x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ll += v[i].y == 0.f ? 0.f : v[i].y * ex2_approx(v[i].x - mm);
+      fin[r] = make_float2(mm, ll);
       const float alpha = l_last == 0.f ? 0.f : ex2_approx(m_last - mm);
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
@@ -471,22 +478,19 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         const int rr = rank * share + i / (HD / 4), d = (i % (HD / 4)) * 4;
         const int idx = (int)blockIdx.x * TB + rr / p.G, hd = (int)blockIdx.z * p.G + rr % p.G;
         if (rr >= rows_tile || idx >= cur.ntok) continue;
-        float m = -INFINITY, ll = 0.f, f[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint32_t mrow = tc::smem_u32(&ml[rr]);
+        float f[4] = {0.f, 0.f, 0.f, 0.f};
+        const float2 row = fin[rr];
         const uint32_t orow = so + (uint32_t)(rr * HD * 4) + (((uint32_t)(d / 4) ^ (uint32_t)(rr & (HD / 4 - 1))) * 16);
-        for (int k = 0; k < cl; ++k) {
-          const float2 v = ld_cluster_f2(tc::map_to_rank(mrow, (uint32_t)k));
-          if (v.y != 0.f) m = fmaxf(m, v.x);
-        }
-#pragma unroll 4
-        for (int k = 0; k < cl; ++k) {
-          const float2 v = ld_cluster_f2(tc::map_to_rank(mrow, (uint32_t)k));
-          ll += v.y == 0.f ? 0.f : v.y * ex2_approx(v.x - m);
-          const float4 q = ld_cluster_f4(tc::map_to_rank(orow, (uint32_t)k));
-          f[0] += q.x; f[1] += q.y; f[2] += q.z; f[3] += q.w;
+        float4 q[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          q[k] = k < cl ? ld_cluster_f4(tc::map_to_rank(orow, (uint32_t)k)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          f[0] += q[k].x; f[1] += q[k].y; f[2] += q[k].z; f[3] += q[k].w;
         }
         const int64_t dest = p.part_o ? (int64_t)(part / cl) * p.T * p.Hq + (int64_t)idx * p.Hq + hd : -1;
-        store_row<4>(p, dest, idx, hd, d, f, m, ll);
+        store_row<4>(p, dest, idx, hd, d, f, row.x, row.y);
       }
       tc::cluster_sync_all();                                                 // no CTA leaves while its memory is read
     }
