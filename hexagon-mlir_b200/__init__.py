@@ -1,5 +1,7 @@
 """hexb200: the hexagon-mlir kernel set (row softmax, LayerNorm, RMSNorm, fp16 matmul,
-flash-attention forward, decoder block stack) as hand-written sm_100a CUDA kernels behind a C ABI.
+flash-attention forward, decoder block stack) as hand-written sm_100a CUDA kernels behind a C ABI, and the
+operators of a serving step over a paged key/value cache (ops.qk_norm_rope, kv_cache_append,
+shared_prefix_attention, sample_tokens).
 
     import hexb200
     hexb200.kernels.softmax_kernel[(4,)](x, out, NUM_ROWS=r, NUM_COLS=c, BLOCK_SIZE=b)   # reference signature

@@ -1,6 +1,7 @@
 /*
  * hexb.h -- C ABI of libhexb200: the hexagon-mlir kernel set (row softmax, LayerNorm, RMSNorm,
- * fp16 matmul, flash-attention forward, decoder block stack) as hand-written sm_100a CUDA kernels.
+ * fp16 matmul, flash-attention forward, decoder block stack) as hand-written sm_100a CUDA kernels, and the
+ * operators of a serving step over a paged key/value cache.
  *
  * Conventions (all entry points):
  *   - plain pointers and sizes, no C++ or torch types; every function returns an int status
@@ -309,6 +310,7 @@ int hexb_kv_cache_append(int dtype, const void *k, const void *v, void *k_cache,
  * (ceil(prefix_len / page_size) entries).  table_width 0: no own keys; prefix_len 0: no prefix.  Lengths, tables and
  * offsets are read on the device by every launch, so a captured graph follows them; a page outside the cache
  * reads as zeros, a length beyond the table is cut, and both make hexb_device_status report HEXB_ERR_BAD_ARG.
+ * Values that some new token of a sequence sees and another does not must be finite (their weight there is 0).
  * max_q: the usual number of new tokens of a sequence, for the launch shape only (0: T / B); any value is right.
  * Q, Out, caches: 16-byte aligned, strides multiples of 8 elements.  Out may be Q.
  * The workspace (see the query; 0 bytes: none) holds nothing between calls; calls that overlap need their own. */
