@@ -11,8 +11,8 @@
 //
 // Every element is read once and written once: the bound is the memory traffic, and for a decode step's few
 // rows the latency of one dependent load.  A row is held by a group of lanes (16 bytes a lane), so the mean
-// is a few shuffles; the sines and cosines depend on (token, pair) only and are computed once per CTA
-// into shared memory, then used by all heads of its tokens.
+// is a few shuffles; the sines and cosines depend on (token, pair) only and are formed once for all heads that a group
+// of lanes walks (in the fallback for odd sizes: once per CTA, in shared memory).
 //
 // The angle of a far position: a 32-bit product of position and frequency is off by up to 2^-24 * 130000 = 0.008 rad
 // at position 130000, so it is formed in 64-bit fixed point and rounded to 32 bits as a fraction of a turn.
