@@ -501,7 +501,8 @@ struct Row {
     __syncthreads();
     int limit = b_k;                              // of what any filter but top-p keeps
     if (min_p > 0.0f) {
-      const float d = -log2f(min_p) / scale32;    // the first difference that min_p drops, to 32 bits
+      // the first difference that min_p drops, to 32 bits (min_p = 1 keeps what 64 bits do not tell from 1)
+      const float d = fmaxf(-log2f(min_p), 4e-16f) / scale32;
       limit = min(limit, (int)fminf(d * f_bin, (float)(NB - 4)) + 2);
     }
     // the mass that top-p takes its share of is top-k's, if there is one: then the list has to hold that
@@ -1021,7 +1022,7 @@ sample_kernel(const Params p) {
     r.top = (double)r.m;
     r.scale32 = (float)c;
     if (top_k >= p.V) top_k = 0;
-    r.v_min = (float)((double)r.m - 1000.0 / c);
+    r.v_min = fmaxf((float)((double)r.m - 1000.0 / c), -3.402823466e38f);   // never -inf: what is masked weighs nothing
     if (r.m == INFINITY) {        // weight 1 for its like, 0 for any other: as if both were the largest finite value
       r.infinite = true;
       r.m = 3.402823466e38f;

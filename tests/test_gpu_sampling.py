@@ -171,6 +171,22 @@ def test_extreme_temperatures(temp):
     compare(x, [0.1, 0.6, 0.5, 0.99], [temp] * 4, [0, 0, 500, 0], [1.0, 0.9, 0.9, 0.3], [0.0, 0.0, 0.0, 0.2])
 
 
+@pytest.mark.parametrize("temp", [1e36, 3e38, float("inf")])
+@pytest.mark.parametrize("rows", [2, 160])
+def test_temperatures_that_level_every_logit(rows, temp):
+    # the weights of all finite logits are 1 to 64 bits; masked places stay out
+    V = 4099
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, V, generator=g)
+    x[:, ::3] = -float("inf")
+    x[:, 1::7] = float("nan")
+    x = x.to(dev)
+    for top_k, top_p, min_p in ((0, 1.0, 0.0), (0, 0.5, 0.0), (100, 1.0, 0.0), (2000, 0.25, 0.5), (0, 1.0, 1.0), (0, 0.5, 1.0),
+                                 (100, 1.0, 1.0), (2000, 1.0, 1.0)):
+        u = np.random.default_rng(7).random(rows, dtype=np.float32)
+        compare(x, u, [temp] * rows, [top_k] * rows, [top_p] * rows, [min_p] * rows)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_strided_rows_of_any_alignment(dtype):
     g = torch.Generator().manual_seed(5)
