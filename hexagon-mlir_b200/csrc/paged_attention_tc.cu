@@ -354,8 +354,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             tc::tmem_st_32x32(tO + lane_off + (uint32_t)(c * 32), o);
           }
         }
-        // a row that has seen no key keeps m_ref = -inf: its weights must come out 0, not NaN
-        const float neg_m = SEQ && m_ref == -INFINITY ? 0.f : -m_ref;
+        // a row that has seen no key, or only infinite ones, keeps m_ref = -inf: its weights must come out 0, not NaN
+        const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;
         const float2 neg_m2 = make_float2(neg_m, neg_m);
         float2 l0 = make_float2(0.f, 0.f), l1 = make_float2(0.f, 0.f);
 #pragma unroll

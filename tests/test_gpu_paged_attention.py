@@ -191,6 +191,40 @@ def test_rising_scores_over_a_long_prefix():
     check(out, q, kc, vc, prefix_pages, P, None, [0] * 200, [1] * 200)
 
 
+@pytest.mark.parametrize("D,G", [(64, 4), (128, 4), (80, 4), (128, 1)])
+def test_keys_of_infinite_scores(D, G):
+    """Keys at -inf in a column where every query is positive weigh nothing, whole key ranges of them too."""
+    P, B, Hkv = 1500, 24, 2
+    prefix_pages, table, pages = layout(P, [70] * B, 16, 4)
+    kc, vc = pool(pages, 16, Hkv, D, 5)
+    rows = kc.view(-1, Hkv, D)
+    slots = (prefix_pages.long()[:, None] * 16 + torch.arange(16, device=dev)).flatten()
+    rows[slots[:900], :, 0] = -float("inf")
+    rows[slots[1400:1440], :, 0] = -float("inf")
+    kc[table[:, :2].long().flatten(), :, :, 0] = -float("inf")
+    q = torch.randn(B, Hkv * G, D, device=dev, generator=torch.Generator(device=dev).manual_seed(3)).half()
+    q[..., 0] = 0.5
+    out = torch.empty_like(q)
+
+    def same_as_without_them(own):
+        # the keys that count, as sequences of their own in pages of one slot
+        for b in range(B if own else 1):
+            k = torch.cat([gather(kc, prefix_pages, P)] + ([gather(kc, table[b], 70)] if own else []))
+            v = torch.cat([gather(vc, prefix_pages, P)] + ([gather(vc, table[b], 70)] if own else []))
+            left = ~k[:, 0, 0].isinf()
+            k, v = k[left].half()[:, None], v[left].half()[:, None]
+            n = k.shape[0]
+            assert n == (P - 940 + 38 if own else P - 940)
+            some = slice(b, b + 1) if own else slice(0, B)
+            check(out[some], q[some], k, v, torch.arange(n, device=dev), n, None, [0] * (1 if own else B), [1] * (1 if own else B))
+
+    ops.shared_prefix_attention(q, kc, vc, out, prefix_pages, P)
+    same_as_without_them(False)
+    ln = torch.full((B,), 70, dtype=torch.int32, device=dev)
+    ops.shared_prefix_attention(q, kc, vc, out, prefix_pages, P, table, ln)
+    same_as_without_them(True)
+
+
 def test_in_place_views_and_a_second_stream():
     Hq, Hkv, D = 8, 2, 128
     prefix_pages, table, pages = layout(300, [20, 30, 70], 16, 9)
