@@ -636,7 +636,7 @@ static int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo :
 static Plan make_plan(const hexb_paged_attention_desc *d, int sm_count) {
   Plan pl = {};
   const int64_t G = d->Hq / d->Hkv, capacity = d->table_width * d->page_size;
-  const int64_t mq = d->max_q > 0 ? d->max_q : ceil_div(d->T, d->B);
+  const int64_t mq = d->max_q > 0 ? clamp64(d->max_q, 1, d->T) : ceil_div(d->T, d->B);
   const int64_t pblocks = ceil_div(d->prefix_len, 64), oblocks = ceil_div(capacity, 64);
   // What TMA can address: page pieces of at least the 8 rows of a swizzle atom, no stride of 0.
   // The tensor-core forms want besides: a positive scale, and enough rows to fill half of a 128-row tile; below that the
@@ -736,8 +736,9 @@ static int check_desc(const hexb_paged_attention_desc *d) {
     return HEXB_ERR_BAD_ARG;
   if (d->T == 0 || d->Hq == 0 || d->B == 0 || d->D == 0) return HEXB_OK;
   if (d->Hkv == 0 || d->Hq % d->Hkv || (!d->q_offsets && d->T != d->B)) return HEXB_ERR_BAD_ARG;
-  if (d->D % 8 || d->D > 256 || d->Hkv > 65535 || d->T > (1 << 24) || d->T * (d->Hq / d->Hkv) > (1 << 30) ||
-      d->B > (1 << 20) || d->prefix_len > (1 << 30) || d->page_size > (1 << 30) || d->num_pages > 0x7fffffff ||
+  if (d->D % 8 || d->D > 256 || d->Hkv > 65535 || d->Hq > (1 << 30) || d->T > (1 << 24) ||
+      d->T * (d->Hq / d->Hkv) > (1 << 30) || d->T * d->Hq > ((int64_t)1 << 32) || d->B > (1 << 20) ||
+      d->prefix_len > (1 << 30) || d->page_size > (1 << 30) || d->num_pages > 0x7fffffff ||
       d->table_width > (1 << 30) / d->page_size)
     return HEXB_ERR_UNSUPPORTED;
   return HEXB_OK;

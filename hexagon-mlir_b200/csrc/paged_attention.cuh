@@ -178,10 +178,10 @@ __device__ __forceinline__ void find_stretch(const Params &p, int rows, long lon
   }
   c.b = s_b;
   enter(p, rows, c);
-  const int off = (int)(s_off % ((long long)c.nb * c.nt)), tile_head = off / c.nb;
-  c.h = (int)(s_off / ((long long)c.nb * c.nt));
-  c.j = off - tile_head * c.nb;
-  c.tile = tile_head;
+  const long long tiles = s_off / c.nb;     // of all key heads
+  c.j = (int)(s_off - tiles * c.nb);
+  c.h = (int)(tiles / c.nt);
+  c.tile = (int)(tiles - (long long)c.h * c.nt);
 }
 
 // Where blocks [j0, j1) of the cursor's tile leave their result.  `tile_first`: the tile's first unit in the list.

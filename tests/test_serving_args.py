@@ -63,6 +63,16 @@ def test_paged_attention_status_codes():
     assert lib.hexb_paged_attention_workspace_bytes(C.byref(desc(D=60))) == 0
 
 
+def test_sizes_past_32_bits_are_refused_or_cut():
+    lib, call = hexb200.load(), lambda **k: hexb200.load().hexb_paged_attention_f16(C.byref(desc(**k)), None, 0, None)
+    assert call(T=1 << 24, B=1 << 20, q_offsets=64, Hq=1 << 15, Hkv=1 << 15) == -2       # rows
+    assert call(Hq=1 << 40, Hkv=1 << 12) == -2 and call(T=1 << 40, B=1 << 40) == -2
+    # a hint of any size means no more than all tokens of the call
+    need = lambda **k: lib.hexb_paged_attention_workspace_bytes(C.byref(desc(**k)))
+    t = desc().T
+    assert need(max_q=(1 << 63) - 1) == need(max_q=t) == need(max_q=1 << 40)
+
+
 def meta(*shape, dtype=torch.float16):
     """A tensor that is refused before its data or device matter."""
     class Fake:
