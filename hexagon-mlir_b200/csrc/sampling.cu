@@ -33,8 +33,9 @@ typedef unsigned long long u64;
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int NB = 2048;           // histogram bins
 constexpr int CAP = 4096;          // list entries
-constexpr int SHORT = 1024;        // of a list that is ranked by counting, and in which all the rest may happen
+constexpr int SHORT = 1024;        // of a list in which all the rest may happen
 constexpr int MAXC = 8;
+constexpr int WIDTHS = 3;          // windows around the guess: 1, 4 and 16 bins to either side
 constexpr int kLevelBits = 10, kLevels = 1 << kLevelBits;  // of the exponential's table
 constexpr uint32_t kNoCut = 0x007fffffu;  // key of -inf
 
@@ -78,7 +79,7 @@ struct Shared {
   float fscan[WARPS];
   unsigned long long before;
   uint32_t bin_count, n;            // list length
-  int found_index, bin, winner, b_k, b_p, b_last, n_last, n_first, n_guess, guessed;
+  int found_index, bin, winner, b_k, b_p, b_last, n_last, n_first[WIDTHS], n_guess[WIDTHS], guessed;
   uint32_t before_k;
   Cut cut;
   int cut_ok;
@@ -442,7 +443,7 @@ struct Row {
   // Leaves: b_k, before_k  bin of the k-th logit and the count before it
   //         b_p            guess of the bin where p of the mass (of what top-k leaves) is reached
   //         b_last         the last bin that the list needs, n_last logits up to it; guessed: b_p set it
-  //         n_first, n_guess   logits before bin b_p - 1, and up to bin b_p + 1
+  //         n_first, n_guess   logits before bin b_p - 4^i, and up to bin b_p + 4^i
   __device__ void plan(const Cut &in, int top_k, float top_p, float min_p, float lowest) {
     // (a sample that is all masked, or all the maximum, says nothing about the width)
     const float range = lowest < m ? fminf(m - lowest, 32.0f) : 32.0f;
@@ -456,7 +457,8 @@ struct Row {
     if (threadIdx.x == 0) {
       s.b_k = s.b_p = NB - 1;
       s.before_k = 0;
-      s.n_last = s.n_first = s.n_guess = 0;
+      s.n_last = 0;
+      for (int i = 0; i < WIDTHS; ++i) s.n_first[i] = s.n_guess[i] = 0;
     }
     cluster_barrier();
     const uint4 c4 = bins4(0);
@@ -482,6 +484,8 @@ struct Row {
       for (int i = 0; i < 4; ++i) {
         const float centre = f_bin > 0.f ? ((float)(b0 + i) + 0.5f) / f_bin : 0.f;
         w[i] = b0 + i <= b_k ? (float)c[i] * exp2f(-centre * scale32) : 0.f;
+        // the maximum, which may hold most of the mass, weighs 1: half a bin off, it would move the guess by many bins
+        if (b0 + i == 0) w[i] += 1.0f - w[i] / (float)c[i];
         sum += w[i];
       }
       float e = exclusive<float>(sum, s.fscan);
@@ -510,10 +514,14 @@ struct Row {
     u64 e = before;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (b0 + i == s.b_p - 1) s.n_first = (int)e;
+#pragma unroll
+      for (int k = 0; k < WIDTHS; ++k)
+        if (b0 + i == s.b_p - (1 << 2 * k)) s.n_first[k] = (int)e;
       e += c[i];
       if (b0 + i == last) s.n_last = (int)e;
-      if (b0 + i == min(s.b_p + 1, NB - 1)) s.n_guess = (int)e;
+#pragma unroll
+      for (int k = 0; k < WIDTHS; ++k)
+        if (b0 + i == min(s.b_p + (1 << 2 * k), NB - 1)) s.n_guess[k] = (int)e;
     }
     if (threadIdx.x == 0) {
       s.b_last = last;
@@ -561,33 +569,24 @@ struct Row {
       at += __popc(who[e]);
     }
   }
-  // Sorts the list, descending (all threads of CTA 0).  Entries differ, so a short list is ranked by counting the larger
-  // ones (300 entries: 4 thousand cycles; the bitonic network takes 12, its steps are all latency).
+  // Sorts the list, descending (all threads of CTA 0).  Entries differ, so a short list -- one entry a thread -- is ranked by
+  // counting the larger ones (300 entries: 4 thousand cycles; the bitonic network takes 12, its steps are all latency).
+  // The count grows with the square: 1000 entries took longer than the network.
   __device__ void sort(u64 *a, int n) {
-    if (n <= SHORT) {
-      constexpr int PER = SHORT / THREADS;
-      u64 mine[PER];
-      int larger[PER];
-#pragma unroll
-      for (int k = 0; k < PER; ++k) {
-        mine[k] = threadIdx.x + k * THREADS < n ? a[threadIdx.x + k * THREADS] : 0;
-        larger[k] = 0;
-      }
+    if (n <= THREADS) {
+      const u64 mine = threadIdx.x < n ? a[threadIdx.x] : 0;
+      int larger = 0;
       if (threadIdx.x == 0 && (n & 1)) a[n] = 0;
       __syncthreads();
-#pragma unroll
-      for (int k = 0; k < PER; ++k) {
-        if (warp * 32 + k * THREADS >= n) break;       // no entry in this warp
+      if (warp * 32 < n) {                             // else no entry in this warp
 #pragma unroll 4
         for (int i = 0; i < n; i += 2) {
           const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(a + i);
-          larger[k] += (q.x > mine[k]) + (q.y > mine[k]);
+          larger += (q.x > mine) + (q.y > mine);
         }
       }
       __syncthreads();
-#pragma unroll
-      for (int k = 0; k < PER; ++k)
-        if (threadIdx.x + k * THREADS < n) a[larger[k]] = mine[k];
+      if (threadIdx.x < n) a[larger] = mine;
       __syncthreads();
       return;
     }
@@ -737,10 +736,10 @@ struct Row {
     }
     return broadcast(cut);
   }
-  // p of the mass: guessed to lie in bin b_p or beside it.
+  // p of the mass: guessed to lie in bin b_p, or at most `width` bins from it.
   // With one CTA a row it also leaves what draw_above needs: `above`, this lane's sum over the bins before those.
-  __device__ bool refine_p(Cut &cut, float top_p, double &above) {
-    const int lo = s.b_p - 1, hi = s.b_p + 1;
+  __device__ bool refine_p(Cut &cut, float top_p, int width, double &above) {
+    const int lo = s.b_p - width, hi = s.b_p + width;
     list_reset();
     double sum = 0.0, cta[C];
     above = 0.0;
@@ -1039,10 +1038,15 @@ sample_kernel(const Params p) {
         if (!drawn) token = -1;
       }
       if (!drawn) {
-        const int n_p = s.n_guess - s.n_first;   // logits around the guess
+        // logits around the guess: the widest window whose list is ranked quickly
+        int width = 1, n_p = s.n_guess[0] - s.n_first[0];
+        for (int k = 1; k < WIDTHS && s.n_guess[k] - s.n_first[k] <= THREADS; ++k) {
+          width = 1 << 2 * k;
+          n_p = s.n_guess[k] - s.n_first[k];
+        }
         if (top_k > 0 && !r.refine_k(cut, top_k)) cut = r.template descend<false>(cut, (double)top_k, 0.0);
         double above = 0.0;
-        const bool refined = top_p < 1.0f && n_p <= CAP && r.refine_p(cut, top_p, above);
+        const bool refined = top_p < 1.0f && n_p <= CAP && r.refine_p(cut, top_p, width, above);
         if (refined && C == 1 && (min_p <= 0.0f || r.min_p_key(min_p) <= cut.key)) {
           token = r.draw_above(cut, above, u);
           if (r.lane) token = -1;
