@@ -181,7 +181,13 @@ struct Row {
 #pragma unroll
     for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
     if (top < low) return;
+    // Behind the cut's index the cut's equals are out; few vectors hold one (256 rows, k = 40000 of 128000: 150 -> 146 us).
+    bool tie = false;
     if (i0 + E - 1 > c.index) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) tie = tie || x[e] == at;
+    }
+    if (tie) {
       double w[E];
       weigh(c, x, i0, w);
 #pragma unroll
