@@ -173,7 +173,7 @@ struct Row {
         if (x[e] == at && i0 + e > c.index) w[e] = 0.0;
     }
   }
-  // sum += their sum; and, of those less deep than `upper` bins, above += it.
+  // sum += their sum; and, of those above the value `upper`, above += it.
   template <bool ABOVE>
   __device__ __forceinline__ void add_weights(const Cut &c, const float (&x)[E], int i0, double &sum, float upper, double &above) const {
     const float at = value_of(c.key), low = fmaxf(at, v_min);
@@ -193,7 +193,7 @@ struct Row {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         sum += w[e];
-        if (ABOVE && depth(x[e]) < upper) above += w[e];
+        if (ABOVE && x[e] > upper) above += w[e];
       }
       return;
     }
@@ -201,7 +201,7 @@ struct Row {
     for (int e = 0; e < E; ++e) {
       const double w = weight_above(x[e]);
       if (x[e] >= low) sum += w;
-      if (ABOVE && x[e] >= low && depth(x[e]) < upper) above += w;
+      if (ABOVE && x[e] >= low && x[e] > upper) above += w;
     }
   }
   // Lowest key whose weight is at least min_p: weights do not fall as keys rise.
@@ -220,6 +220,24 @@ struct Row {
   }
   // Does not fall as v falls.  (bin_of(v) < b, for b < NB, is depth(v) < b.)
   __device__ __forceinline__ float depth(float v) const { return (m - v) * f_bin; }
+  // The largest value at least `bin` deep; -inf if no finite one is.  Passes compare with it instead of forming every depth.
+  // Whole warps call it: one round around the estimate, and if that misses, rounds that cut the range of keys by 33.
+  __device__ float value_at(int bin) const {
+    if (bin <= 0) return m;
+    uint32_t lo = kNoCut, hi = key_of(m);            // lo: deep enough, or the key of -inf; hi: not
+    const uint32_t near = key_of(m - (float)bin / f_bin) - 16 + lane;
+    const bool in = near > lo && near < hi;
+    const unsigned fits = __ballot_sync(0xffffffffu, in && depth(value_of(near)) >= (float)bin);
+    if (__all_sync(0xffffffffu, in) && (fits & 1u) && !(fits >> 31)) return value_of(near - lane + __popc(fits) - 1);
+    while (hi - lo > 1) {
+      const uint32_t step = (hi - lo - 1) / 33 + 1, k = lo + step * (lane + 1);
+      const bool deep = k > lo && k < hi && hi - lo > step * (lane + 1) && depth(value_of(k)) >= (float)bin;
+      const uint32_t n = __popc(__ballot_sync(0xffffffffu, deep));
+      lo += step * n;
+      hi = min(hi - lo, step) + lo;
+    }
+    return value_of(lo);
+  }
   __device__ __forceinline__ int bin_of(float v) const { return (int)fminf(depth(v), (float)(NB - 1)); }
   // The elements of vector v, and the row index of the first.  NaN, and places outside the slice, come as -inf.
   __device__ __forceinline__ int vector(int v, float (&x)[E]) const {
@@ -537,18 +555,18 @@ struct Row {
   }
 
   // ------------------------------------------------------------ the list
+  // The value behind the last of bin `bin`: a list of bins up to that one takes what lies above.
+  __device__ __forceinline__ float behind(int bin) const { return bin >= NB - 1 ? -INFINITY : value_at(bin + 1); }
   __device__ __forceinline__ void list_reset() {
     if (threadIdx.x == 0) s.n = 0;
     cluster_barrier();
   }
-  // Appends the elements in bins [lo, hi] that the cut keeps to the list of CTA 0; the whole warp calls it.
-  __device__ __forceinline__ void append(const Cut &c, int lo, int hi, const float (&x)[E], int i0) {
-    const float from = (float)lo, to = hi >= NB - 1 ? INFINITY : (float)(hi + 1);
+  // Appends the elements above `below`, up to `from`, that the cut keeps to the list of CTA 0; the whole warp calls it.
+  __device__ __forceinline__ void append(const Cut &c, float from, float below, const float (&x)[E], int i0) {
     bool take[E], any = false;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float d = depth(x[e]);
-      take[e] = d >= from && d < to && x[e] > -INFINITY;
+      take[e] = x[e] <= from && x[e] > below;
       any = any || take[e];
     }
     if (!__any_sync(0xffffffffu, any)) return;       // most vectors hold none
@@ -669,8 +687,9 @@ struct Row {
     double sum = 0.0, cta[C];
     const bool total_needed = top_p < 1.0f && top_k <= 0;
     const Cut all = {kNoCut, 0x7fffffff};
+    const float below = behind(last);
     each([&](const float (&x)[E], int i) {
-      append(all, 0, last, x, i);
+      append(all, m, below, x, i);
       double none;
       if (total_needed) add_weights<false>(all, x, i, sum, 0.f, none);
     });
@@ -728,7 +747,8 @@ struct Row {
     const int rank_in = top_k - (int)s.before_k;     // 1 ..
     list_reset();
     const Cut all = {kNoCut, 0x7fffffff};
-    each([&](const float (&x)[E], int i) { append(all, b, b, x, i); });
+    const float from = value_at(b), below = behind(b);
+    each([&](const float (&x)[E], int i) { append(all, from, below, x, i); });
     cluster_barrier();
     if (rank == 0) {
       const int n = (int)min(s.n, (uint32_t)CAP);
@@ -749,9 +769,10 @@ struct Row {
     list_reset();
     double sum = 0.0, cta[C];
     above = 0.0;
+    const float from = value_at(lo), below = behind(hi);
     each([&](const float (&x)[E], int i) {
-      append(cut, lo, hi, x, i);
-      add_weights<true>(cut, x, i, sum, (float)lo, above);
+      append(cut, from, below, x, i);
+      add_weights<true>(cut, x, i, sum, from, above);
     });
     const double total = cluster_total(sum, cta);
     const double over = cluster_total(above, cta);
