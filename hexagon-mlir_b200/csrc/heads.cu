@@ -103,8 +103,8 @@ __device__ __forceinline__ int64_t load_slot(const Params &p, int64_t token) {
 
 // Vector form.  LPR lanes hold one row, NV 16-byte vectors each (vector v sits in lane v % LPR, register v / LPR).
 // A CTA takes tokens_per_cta tokens; a token's heads (of both tensors, in one row) are dealt to 1 << gpt_shift groups
-// of lanes.  Instruction issue, not memory, bounds this kernel (350 instructions a row with the addresses and the
-// rotation formed anew for each: 80 us where the traffic takes 21), so what the rows of a group share is set up
+// of lanes.  Instruction issue bounds a kernel that forms addresses and rotation anew for each row (46 M warp instructions,
+// 86 us for the append below, now 14 M, where the traffic takes 21 us), so what the rows of a group share is set up
 // once: the addresses advance by a constant, and the linear map of a row
 //   y_e = rstd * (A_e x_e + B_e x_partner(e)),   A = w cos,  B = -+ w_partner sin
 // sits in registers -- two fused operations an element besides the mean.  AHEAD rows of a group are under way, the first
