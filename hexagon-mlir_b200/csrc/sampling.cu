@@ -23,7 +23,7 @@
 // Few rows: a cluster of CTAs owns a row, each with its slice in shared memory, and exchanges maxima, sums and
 // histograms through distributed shared memory; a step costs latency only.  Many rows: one CTA a row, two an SM, the
 // passes read the row from L2; instruction issue is the bound (256 rows of 128000 fp16, 65 MB, 10 us of memory: 24 us for
-// the maximum alone, 79 without filters, 157 with top-p).
+// the maximum alone, 79 without filters, 149 with top-p).
 #include "tc_sm100.cuh"
 
 namespace hexb {
