@@ -531,8 +531,10 @@ struct Row {
     int limit = b_k;                              // of what any filter but top-p keeps
     if (min_p > 0.0f) {
       // the first difference that min_p drops, to 32 bits (min_p = 1 keeps what 64 bits do not tell from 1)
-      const float d = fmaxf(-log2f(min_p), 4e-16f) / scale32;
-      limit = min(limit, (int)fminf(d * f_bin, (float)(NB - 4)) + 2);
+      const float d = fmaxf(-log2f(min_p), 4e-16f) / scale32, reach = d * f_bin;
+      // behind the range all lie in the last bin, so a reach past it is no limit (the range is a sample's: in a row masked
+      // but for a few logits it may be a part of what min_p keeps)
+      if (reach < (float)(NB - 4)) limit = min(limit, (int)reach + 2);
     }
     // the mass that top-p takes its share of is top-k's, if there is one: then the list has to hold that
     const int last = top_p < 1.0f ? (top_k > 0 ? b_k : min(limit, s.b_p + 1)) : limit;

@@ -251,3 +251,32 @@ def test_another_stream_graph_and_empty():
     ops.sample_tokens(x.cpu(), u.cpu(), host, top_k=torch.full((4,), 40, dtype=torch.int32))
     assert torch.equal(host, got.cpu())
     assert hexb200.device_status() == 0
+
+
+def test_min_p_keeps_logits_behind_the_histograms_range():
+    """A constrained vocabulary: the first places of a row do not show how far its few logits reach."""
+    V, at = 60000, [0, 1, 1000, 2000, 3000]
+    row = torch.full((V,), -float("inf"), dtype=torch.float16)
+    row[at] = torch.tensor([5.0, 4.5, 4.0, 3.5, 3.0], dtype=torch.float16)
+    for rows in (1, 80):
+        x = row.to(dev).expand(rows, V)
+        for top_k, top_p in ((50, 1.0), (0, 0.99), (50, 0.99)):
+            for u in np.linspace(0.01, 0.99, 80, dtype=np.float32).reshape(-1, rows)[::8 if rows == 1 else 1]:
+                compare(x, u, [1.0] * rows, [top_k] * rows, [top_p] * rows, [0.05] * rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("vocab", [50257, 128000])
+@pytest.mark.parametrize("rows", [1, 160])
+def test_min_p_with_few_allowed_tokens(rows, vocab, dtype):
+    g = torch.Generator().manual_seed(vocab + rows)
+    r = np.random.default_rng(vocab)
+    for trial in range(16 if rows == 1 else 1):
+        x = torch.full((rows, vocab), -float("inf"))
+        for i in range(rows):
+            at = torch.randperm(vocab, generator=g)[:(2, 5, 10, 20)[(i + trial) % 4]]
+            x[i, at] = torch.randn(len(at), generator=g) * 2
+        x = x.to(dtype).to(dev)
+        for top_k, top_p in ((50, 1.0), (0, 0.99), (8, 0.9), (0, 1.0)):
+            compare(x, r.random(rows, dtype=np.float32), r.choice([0.7, 1.0], rows), [top_k] * rows, [top_p] * rows,
+                    r.choice([0.02, 0.05, 0.1], rows))
