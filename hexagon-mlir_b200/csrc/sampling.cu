@@ -121,7 +121,7 @@ struct Row {
   float m, f_bin;         // maximum; bins per unit of value
   double top, scale;      // the maximum; kLevels * log2(e) / T
   float scale32, v_min;
-  bool infinite;          // the maximum is: the elements come as the largest finite value, or as -inf
+  bool infinite;          // the maximum is: the elements come as 0 (its like), or as -inf
   int flip;
 
   __device__ Row(const Params &p_, Shared &s_) : p(p_), s(s_), infinite(false), flip(0) {}
@@ -1052,11 +1052,11 @@ sample_kernel(const Params p) {
     r.scale32 = (float)c;
     if (top_k >= p.V) top_k = 0;
     r.v_min = fmaxf((float)((double)r.m - 1000.0 / c), -3.402823466e38f);   // never -inf: what is masked weighs nothing
-    if (r.m == INFINITY) {        // weight 1 for its like, 0 for any other: as if both were the largest finite value
+    if (r.m == INFINITY) {        // weight 1 for its like, 0 for any other: they come as 0, the others as -inf
       r.infinite = true;
-      r.m = 3.402823466e38f;
-      r.top = (double)r.m;
-      r.v_min = r.m;
+      r.m = 0.0f;                 // a value of either type: the key's low bits are those of a widened fp16 value
+      r.top = 0.0;
+      r.v_min = 0.0f;
     }
     Cut cut = {kNoCut, 0x7fffffff};
     bool drawn = false;

@@ -280,3 +280,19 @@ def test_min_p_with_few_allowed_tokens(rows, vocab, dtype):
         for top_k, top_p in ((50, 1.0), (0, 0.99), (8, 0.9), (0, 1.0)):
             compare(x, r.random(rows, dtype=np.float32), r.choice([0.7, 1.0], rows), [top_k] * rows, [top_p] * rows,
                     r.choice([0.02, 0.05, 0.1], rows))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rows", [2, 160])
+def test_filters_among_thousands_of_infinite_logits(rows, dtype):
+    """+inf logits are equals: the filters keep the lowest indexes of them, finite ones weigh nothing."""
+    V = 20000
+    x = torch.full((rows, V), 3.0, dtype=dtype)
+    x[:, ::5] = -7.0
+    x[:, 1::3] = float("inf")                                       # 6667
+    x = x.to(dev)
+    u = np.resize(np.array([0.0, 0.21, 0.52, 0.999], dtype=np.float32), rows)
+    # 5 by top-k; before the 3334th lie 3333 of 6667, less than half; 1500 of 6000; all with min-p alone
+    for top_k, top_p, min_p, kept in ((5, 1.0, 0.0, 5), (0, 0.5, 0.0, 3334), (6000, 0.25, 0.0, 1500), (6000, 1.0, 0.5, 6000),
+                                      (0, 1.0, 1.0, 6667)):
+        assert call(x, u, [0.8] * rows, [top_k] * rows, [top_p] * rows, [min_p] * rows) == [1 + 3 * int(float(v) * kept) for v in u]
