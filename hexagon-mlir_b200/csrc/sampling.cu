@@ -9,8 +9,9 @@
 // Ties are ordered by index everywhere (the lower one first), so each filter keeps a prefix of one descending order, and
 // a cut in it -- (key, index) -- says all.  NaN and -inf are never chosen; a row with nothing else gives -1.
 //
-// A token is a whole number, so borders decide: weights and sums are formed in 64 bits, or as exact integers (44 bits of
-// the mass), and in an order that does not depend on how the threads run.
+// A token is a whole number, so borders decide: weights (relative error below 2^-37, see weight()) are formed and summed in
+// 64 bits, as floating-point numbers or as integers of at least 60 bits of the mass, and in an order that does not depend on
+// how the threads run.
 //
 // Drawing in index order needs no sorted row.  A histogram of the row's values (one shared-memory atomic a logit) gives
 // the cut of top-k to a bin, and with the bins' weights a guess of the cut of top-p to a few.  Then one pass
@@ -435,16 +436,31 @@ struct Row {
     }
     __syncthreads();
   }
-  // This thread's four bins of the cluster's histogram (0: counts, 1 and 2: the words of the mass).
-  __device__ __forceinline__ uint4 bins4(int which) {
-    const uint32_t *h = which == 0 ? s.count : reinterpret_cast<const uint32_t *>(s.list) + (which - 1) * NB;
+  // This thread's four bins of the cluster's histogram: counts, or the mass (the high words, then the low ones).
+  __device__ __forceinline__ uint4 bins4_of(const uint32_t *h, int r) {
+    return C > 1 ? ld_cluster_u128(peer(h + threadIdx.x * 4, r)) : *reinterpret_cast<const uint4 *>(h + threadIdx.x * 4);
+  }
+  __device__ __forceinline__ uint4 bins4() {
     uint4 c = make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int r = 0; r < C; ++r) {
-      const uint4 v = C > 1 ? ld_cluster_u128(peer(h + threadIdx.x * 4, r)) : *reinterpret_cast<const uint4 *>(h + threadIdx.x * 4);
+      const uint4 v = bins4_of(s.count, r);
       c.x += v.x; c.y += v.y; c.z += v.z; c.w += v.w;
     }
     return c;
+  }
+  __device__ __forceinline__ void mass4(u64 (&v)[4]) {
+    const uint32_t *hi = reinterpret_cast<const uint32_t *>(s.list), *lo = hi + NB;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = 0;
+#pragma unroll
+    for (int r = 0; r < C; ++r) {
+      const uint4 h = bins4_of(hi, r), l = bins4_of(lo, r);
+      v[0] += (u64)h.x << 32 | l.x;
+      v[1] += (u64)h.y << 32 | l.y;
+      v[2] += (u64)h.z << 32 | l.z;
+      v[3] += (u64)h.w << 32 | l.w;
+    }
   }
   // exclusive prefix over the threads of the CTA
   template <typename U>
@@ -486,7 +502,7 @@ struct Row {
       for (int i = 0; i < WIDTHS; ++i) s.n_first[i] = s.n_guess[i] = 0;
     }
     cluster_barrier();
-    const uint4 c4 = bins4(0);
+    const uint4 c4 = bins4();
     const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
     const u64 before = exclusive<u64>((u64)c[0] + c[1] + c[2] + c[3], s.scan);
     const int b0 = threadIdx.x * 4;
@@ -817,14 +833,11 @@ struct Row {
   template <bool MASS>
   __device__ void find_bin(double need) {
     cluster_barrier();  // all histograms are complete
-    const uint4 c4 = bins4(0), h4 = MASS ? bins4(1) : make_uint4(0, 0, 0, 0), l4 = MASS ? bins4(2) : make_uint4(0, 0, 0, 0);
-    const uint32_t cnt[4] = {c4.x, c4.y, c4.z, c4.w}, h[4] = {h4.x, h4.y, h4.z, h4.w}, l[4] = {l4.x, l4.y, l4.z, l4.w};
-    u64 v[4], sum = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = MASS ? ((u64)h[i] << 14) + l[i] : cnt[i];
-      sum += v[i];
-    }
+    const uint4 c4 = bins4();
+    const uint32_t cnt[4] = {c4.x, c4.y, c4.z, c4.w};
+    u64 v[4] = {c4.x, c4.y, c4.z, c4.w};
+    if (MASS) mass4(v);
+    const u64 sum = v[0] + v[1] + v[2] + v[3];
     if (threadIdx.x == 0) s.bin = -1;
     const u64 excl = exclusive<u64>(sum, s.scan);
     // the crossing bin; without one (rounding at the far end) the last bin that holds anything
@@ -865,8 +878,8 @@ struct Row {
     cluster_barrier();  // every CTA has read the histograms
   }
 
-  // The cut of top-k (MASS false: `need` elements) or top-p (MASS true: `need` units of mass; unit = 1 / units): bins of
-  // keys, narrowed until a bin is one key.
+  // The cut of top-k (MASS false: `need` elements) or top-p (MASS true: `need` units of mass; unit = 1 / units, a power of
+  // two, so that equal logits of weight 1 sum exactly): bins of keys, narrowed until a bin is one key.
   template <bool MASS>
   __device__ Cut descend(const Cut &in, double need, double units) {
     constexpr int KS = sizeof(T) == 2 ? 13 : 0;  // a widened fp16 value leaves the low 13 bits of its key alone
@@ -887,9 +900,11 @@ struct Row {
           const uint32_t b = ((hi >> KS) - (k >> KS)) >> sh;
           atomicAdd(&s.count[b], 1u);
           if (MASS) {
+            // 64-bit sums in two words, the low one's carries with the high one: whatever the order, the same integer
             const u64 q = __double2ull_rn(weight(x[e]) * units);
-            atomicAdd(&hi_words[b], (uint32_t)(q >> 14));
-            atomicAdd(&lo_words[b], (uint32_t)(q & 16383u));
+            const uint32_t low = (uint32_t)q;
+            const uint32_t high = (uint32_t)(q >> 32) + (atomicAdd(&lo_words[b], low) + low < low);
+            if (high) atomicAdd(&hi_words[b], high);
           }
         }
       });
@@ -1090,8 +1105,11 @@ sample_kernel(const Params p) {
             double none;
             r.template add_weights<false>(cut, x, i, part, 0.f, none);
           });
-          const double units = 17592186044416.0 / r.cluster_total(part, cta);  // 2^44 in all
-          cut = r.template descend<true>(cut, fmax((double)top_p * 17592186044416.0, 1.0), units);
+          // 2^60 to 2^61 units in all (the largest weighs 1, so the total is at least that): vocab / 2 of them, at most
+          // 2^-33 of the mass at 2^28 logits, bound what rounding the weights to units does
+          const double total = r.cluster_total(part, cta);
+          const double units = __hiloint2double((2 * 1023 + 60 - (__double2hiint(total) >> 20)) << 20, 0);
+          cut = r.template descend<true>(cut, fmax((double)top_p * total * units, 1.0), units);
         }
       }
     }

@@ -296,3 +296,31 @@ def test_filters_among_thousands_of_infinite_logits(rows, dtype):
     for top_k, top_p, min_p, kept in ((5, 1.0, 0.0, 5), (0, 0.5, 0.0, 3334), (6000, 0.25, 0.0, 1500), (6000, 1.0, 0.5, 6000),
                                       (0, 1.0, 1.0, 6667)):
         assert call(x, u, [0.8] * rows, [top_k] * rows, [top_p] * rows, [min_p] * rows) == [1 + 3 * int(float(v) * kept) for v in u]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(1, 1000003), (80, 1000003), (1, 12000001)])
+@pytest.mark.parametrize("with_top_k", [False, True])
+def test_top_p_among_millions_of_equal_logits(rows, vocab, with_top_k, dtype):
+    """Logits 0 at even places and -1 at odd ones: sums of the definition are whole numbers of two weights."""
+    row = torch.zeros(vocab, dtype=dtype)
+    row[1::2] = -1.0
+    n0, n1, w = (vocab + 1) // 2, vocab // 2, float(np.exp(-1.0))
+    top_k, top_p = 0, float(np.float32(0.9))
+    if with_top_k:
+        n1 = n1 * 3 // 4
+        top_k = n0 + n1
+    last = (top_p * (n0 + n1 * w) - n0) / w                          # of the odd places, how many are kept
+    assert 0.05 < last % 1 < 0.95
+    odd = np.arange(vocab) % 2 == 1
+    c1 = np.minimum(np.cumsum(odd), int(np.ceil(last)))
+    cum = np.cumsum(~odd) + c1 * w
+    r = np.random.default_rng(5)
+    u = np.concatenate([[np.float32(1 - 2.0 ** -24), np.float32(0.9999)], r.random(200, dtype=np.float32)]).astype(np.float32)
+    t = u.astype(np.float64) * cum[-1]
+    want = np.searchsorted(cum, t, side="right")
+    far = np.minimum(np.abs(cum[np.minimum(want, vocab - 1)] - t), np.abs(t - cum[want - 1])) > 1e-9 * cum[-1]
+    u, want = u[far], want[far].tolist()
+    x = row.to(dev).expand(rows, vocab)
+    for i in range(0, 8 if rows == 1 else 1):
+        assert call(x, u[i:i + rows], [1.0] * rows, [top_k] * rows, [top_p] * rows, [0.0] * rows) == want[i:i + rows]
