@@ -345,9 +345,9 @@ paged_stream_tma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
     tc::prefetch_tensormap(&tmK);
     tc::prefetch_tensormap(&tmV);
   }
-  // After the call's own tensor-core launch this one need not wait: it does not touch what that one writes, and that
-  // one lets it start only when all that came before is complete.
-  if (!p.follows_prefix) pdl_wait();
+  // Also after the call's own tensor-core launch, whose results this one does not touch: what earlier kernels of the stream
+  // wrote -- queries, lengths, tables, the cache -- is certain to be visible only behind the wait.
+  pdl_wait();
   long long start, stop, per;
   Cursor c;
   find_stretch<160>(p, 16 * RW, start, stop, per, c);   // its barriers also publish the ones set up above
@@ -429,7 +429,6 @@ paged_stream_tma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
       if (threadIdx.x == 0) atomicExch(&g_paged_status, (int)HEXB_ERR_TIMEOUT);
     }
   }
-  pdl_wait();  // whoever waits for this launch waits for the tensor-core launch too
   pdl_launch_dependents();
 }
 
@@ -444,7 +443,7 @@ paged_stream_kernel(const Params p) {
   const uint32_t s0 = (uint32_t)__cvta_generic_to_shared(smem);
   int64_t *offs = reinterpret_cast<int64_t *>(smem + cfg::OFFS);
   const int tid = threadIdx.x, warp = tid >> 5;
-  if (!p.follows_prefix) pdl_wait();
+  pdl_wait();
   long long start, stop, per;
   Cursor cc, cl;                        // the unit being computed, the one whose pages are looked up
   find_stretch<THREADS>(p, 16 * RW, start, stop, per, cc);
@@ -536,7 +535,6 @@ paged_stream_kernel(const Params p) {
     }
     cp_async_wait<0>();
   }
-  pdl_wait();  // whoever waits for this launch waits for the tensor-core launch too
   pdl_launch_dependents();
 }
 
@@ -821,7 +819,6 @@ extern "C" int hexb_paged_attention_f16(const hexb_paged_attention_desc *d, void
     if (int e = paged::tc_launch(p, (int)d->Hkv, false, grid, st)) return e;
   }
   if (pl.stream) {
-    p.follows_prefix = pl.tc_prefix;
     p.stream_prefix = pl.stream_prefix;
     CUtensorMap tm[2];
     if (pl.tma)

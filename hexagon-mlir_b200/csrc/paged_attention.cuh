@@ -33,7 +33,6 @@ struct Params {
   int shared_blocks;                  // blocks of the prefix at the head of every sequence's axis
   int tile_tokens, piece;             // tensor-core form: tokens of a tile, keys of one TMA box
   int cluster;                        // and key ranges of a tile that one cluster joins
-  int follows_prefix;                 // the stream follows the call's tensor-core launch over the prefix
   int nseq;                           // sequences in the stream: B, or 0 without own keys
   int stream_prefix;                  // the stream of key blocks covers the prefix too
 };

@@ -105,7 +105,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   tc::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();
-  // Only now: a successor that starts here may rely on all that came before this kernel, but not on this kernel.
+  // The next launch may take the places of CTAs that are done; it waits for this whole grid before it reads anything.
   pdl_launch_dependents();
   const uint32_t tO = tmem_base + cfg::O_COL;
 

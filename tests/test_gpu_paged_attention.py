@@ -337,3 +337,38 @@ def test_host_tensors_are_staged():
     ln = torch.tensor([9], dtype=torch.int32)
     ops.shared_prefix_attention(q.cpu(), kc.cpu(), vc.cpu(), out, prefix_pages.cpu(), 40, table.cpu(), ln)
     check(out.to(dev), q, kc, vc, prefix_pages, 40, table, [9], [1])
+
+
+@pytest.mark.parametrize("D", [64, 128, 80])
+def test_inputs_written_right_before_the_call(D):
+    """Queries, lengths, tables and own keys that the kernels before it in the stream wrote, step after step."""
+    B, Hq, Hkv, page, P = 70, 8, 2, 16, 700
+    prefix_pages, table, pages = layout(P, [64] * B, page, 3)
+    kc, vc = pool(pages, page, Hkv, D, 3)
+    g = torch.Generator(device=dev).manual_seed(4)
+    own_pages = table.flatten().long()
+    sources, outs = [], []
+    for i in range(6):
+        lens = torch.randint(0, 65, (B,), generator=g, device=dev, dtype=torch.int32)
+        q = torch.randn(B, Hq, D, generator=g, device=dev).half()
+        keys = torch.randn(2, B * 4, page, Hkv, D, generator=g, device=dev).half()
+        sources.append((q, lens, table[torch.randperm(B, generator=g, device=dev)], keys))
+        outs.append(torch.empty_like(q))
+    q, lens, tab = torch.empty_like(sources[0][0]), torch.empty_like(sources[0][1]), torch.empty_like(table)
+
+    def step(i):
+        kc.index_copy_(0, own_pages, sources[i][3][0])
+        vc.index_copy_(0, own_pages, sources[i][3][1])
+        for dst, src in zip((tab, lens, q), (sources[i][2], sources[i][1], sources[i][0])):
+            dst.copy_(src)
+        ops.shared_prefix_attention(q, kc, vc, outs[i], prefix_pages, P, tab, lens)
+
+    for _ in range(20):
+        for i in range(6):
+            step(i)
+    torch.cuda.synchronize()
+    for i in range(6):
+        got = outs[i].clone()
+        step(i)
+        assert torch.equal(outs[i], got)                         # the same, whatever ran before
+        check(got, sources[i][0], kc, vc, prefix_pages, P, sources[i][2], sources[i][1].tolist(), [1] * B)
