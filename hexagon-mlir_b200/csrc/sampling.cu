@@ -919,7 +919,7 @@ struct Row {
         if (MASS) t = ceil((need - (double)before) / (weight(value_of(k)) * units));
         else t = need - (double)before;
         if (!(t > 1.0)) t = 1.0;
-        Cut c = {k, 0x7fffffff};
+        Cut c = {k, k == in.key ? in.index : 0x7fffffff};   // all that were left of the key's equals, or fewer
         if (t < (double)ties) c.index = tie_index(in, k, t);
         return c;
       }

@@ -324,3 +324,16 @@ def test_top_p_among_millions_of_equal_logits(rows, vocab, with_top_k, dtype):
     x = row.to(dev).expand(rows, vocab)
     for i in range(0, 8 if rows == 1 else 1):
         assert call(x, u[i:i + rows], [1.0] * rows, [top_k] * rows, [top_p] * rows, [0.0] * rows) == want[i:i + rows]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rows", [2, 160])
+def test_top_p_of_what_top_k_leaves_of_equal_logits(rows, dtype):
+    """Top-k cuts through thousands of equal logits, and top-p (0.9 of 5) may leave all that top-k did."""
+    V = 12000
+    x = torch.full((rows, V), -1.0, dtype=dtype)
+    x[:, ::2] = 2.0                                                  # 6000
+    x = x.to(dev)
+    u = np.resize(np.array([0.0, 0.21, 0.53, 0.999], dtype=np.float32), rows)
+    for top_k, top_p, min_p, kept in ((5, 0.9, 0.0, 5), (50, 0.99, 0.5, 50), (5000, 0.9999, 0.0, 5000), (5000, 0.5, 0.9, 2500)):
+        assert call(x, u, [0.7] * rows, [top_k] * rows, [top_p] * rows, [min_p] * rows) == [2 * int(float(v) * kept) for v in u]
