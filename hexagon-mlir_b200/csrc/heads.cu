@@ -56,8 +56,9 @@ struct Params {
 // Angles are fractions of a turn in 64-bit fixed point: 2^64 is one turn, a product with the position wraps as an angle
 // does, and no chain of 64-bit floating-point operations delays the first row of a CTA.  The frequency of pair p is
 // 2^64 / (2 pi) * theta^(-2p / rotary_dim): the product of the powers theta^(-2^(b+1) / rotary_dim) over the bits b of p,
-// which the host forms in 64-bit floating point (2^63 is 1): relative error at most 12 * 2^-53, so the angle at position n
-// is good to n * 2^-50 of a turn.
+// which the host forms in 64-bit floating point (2^63 is 1).  A power is off by a relative 2^-52, on a frequency of at most
+// 0.16 turn a position: 11 of them 2^-51 of a turn.  Their truncation to integers and that of the products add at most 3
+// units of 2^-64 of a turn each, whatever is left of the frequency: 2^-58.  So the angle at position n is good to n * 2^-50.
 __device__ __forceinline__ uint64_t frequency(const Params &p, int pr) {
   uint64_t f = 2935890503282001226ull;  // 2^64 / (2 pi)
 #pragma unroll

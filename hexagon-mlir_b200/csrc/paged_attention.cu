@@ -6,8 +6,9 @@
 // partial results: a part holds its row maximum m (base 2, scale folded in), l = sum 2^(s - m) and
 // O = sum 2^(s - m) v, and
 //     out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i,   M = max_i m_i,
-// so the prefix is read once for all queries of the batch instead of once per sequence, and a long axis is cut
-// into parts that run side by side.  Query heads that share a key head (and tokens) form the rows of a tile.
+// so the prefix can be read for a tile of rows from many sequences instead of once per sequence, and a long axis is cut
+// into parts that run side by side.  Query heads that share a key head (and tokens) form the rows of a tile.  From 64 rows
+// a sequence on, a tile holds one sequence alone and reads the prefix itself (make_plan).
 //
 // A row that sees no key (empty sequence, no prefix) gives zeros.  Rows behind the last sequence are not
 // written.  fp32 scores, statistics and sums; P is rounded to fp16 for the second product as in the library's
@@ -637,8 +638,7 @@ static Plan make_plan(const hexb_paged_attention_desc *d, int sm_count) {
   const int64_t mq = d->max_q > 0 ? clamp64(d->max_q, 1, d->T) : ceil_div(d->T, d->B);
   const int64_t pblocks = ceil_div(d->prefix_len, 64), oblocks = ceil_div(capacity, 64);
   // What TMA can address: page pieces of at least the 8 rows of a swizzle atom, no stride of 0.
-  // The tensor-core forms want besides: a positive scale, and enough rows to fill half of a 128-row tile; below that the
-  // key stream, not the products, is what takes the time, and the small tiles of mma.sync read it as fast.
+  // The tensor-core forms want besides: a positive scale, and enough rows to fill half of a 128-row tile.
   pl.piece = (int)(d->page_size & -d->page_size);
   if (pl.piece > 64) pl.piece = 64;
   bool tma_ok = (d->D == 64 || d->D == 128) && pl.piece >= 8;
@@ -651,7 +651,10 @@ static Plan make_plan(const hexb_paged_attention_desc *d, int sm_count) {
   // CTAs for a list of at most `tiles` tiles of at most `blocks` blocks: those that fit the GPU, fewer for a short list
   auto ctas_for = [&](double units, int64_t fit) { return clamp64(units < (double)fit ? (int64_t)units : fit, 1, fit); };
   if (tc_ok && mq * G >= 64 && capacity > 0) {
-    // tiles of one sequence each, over the prefix and its own keys
+    // Tiles of one sequence each, over the prefix and its own keys, from 64 rows a sequence on.  Against the stream (behind
+    // the packed prefix form, if there is a prefix), 8 key heads of 128, G = 4: 16 sequences of 2048 own keys, no prefix, 32
+    // rows each 38.9 us against 43.7, 64 rows 43.9 against 67.4; 64 sequences of 512 behind 8192 shared keys 333 against 159,
+    // 332 against 269, and at 96 rows 345 against 502: a long prefix, which each tile reads for itself, moves the border up.
     pl.seq = true;
     pl.tile_rows = 128;
     const double tiles = (double)(ceil_div(d->T, pl.tile_tokens) + d->B) * d->Hkv;
@@ -661,9 +664,12 @@ static Plan make_plan(const hexb_paged_attention_desc *d, int sm_count) {
   }
   if (d->prefix_len > 0 && tc_ok && d->T * G >= 64) {
     pl.tc_prefix = true;
+    // The prefix by 128-row tiles, from 64 rows on.  Against the stream, 8192 keys, 8 key heads of 128, G = 4: with 512 own
+    // keys a sequence 32 rows 33.3 us against 30.5 (one launch more), 64 rows 36.0 against 38.9, 256 rows 61.8 against 98.3;
+    // the prefix alone 20.0 against 28.8, 20.7 against 33.1, 26.5 against 57.9.
     const int64_t tiles = (int64_t)ceil_div(d->T, pl.tile_tokens) * d->Hkv;
-    // Two CTAs an SM.  (One, so that the stream's CTAs run beside it, takes longer: a single CTA does not keep the tensor
-    // pipe busy.  64 sequences behind 8192 keys 74 us against 65, 128 behind 16385 keys 150 against 118.)
+    // Two CTAs an SM: one does not keep the tensor pipe busy (the prefix alone: 64 sequences behind 8192 keys 29.3 us against
+    // 26.3, 128 behind 16385 keys 82.6 against 50.5).
     const int64_t ranges = clamp64(2 * sm_count / tiles, 1, clamp64((pblocks + 1) / 2, 1, 64));
     for (pl.cluster = 8; pl.cluster > ranges;) pl.cluster /= 2;
     pl.prefix_parts = (int)(ranges / pl.cluster);

@@ -691,7 +691,7 @@ def _indexes(name: str, t, dim: int):
 
 def shared_prefix_attention(q, k_cache, v_cache, out, prefix_pages=None, prefix_len: int = 0, block_table=None,
                             seq_lens=None, q_offsets=None, max_q: int = 0, sm_scale=None) -> None:
-    """Attention of a batch whose sequences share a prefix, over a paged cache; the prefix is read once for all.
+    """Attention of a batch whose sequences share a prefix, over a paged cache that holds the prefix once.
 
     q, out: float16 [tokens, q_heads, D] (out may be q); caches: float16 [num_pages, page_size, kv_heads, D], any
     strides with a unit innermost one; q_heads a multiple of kv_heads (query heads h*G .. h*G+G-1 read key head h);
@@ -701,7 +701,8 @@ def shared_prefix_attention(q, k_cache, v_cache, out, prefix_pages=None, prefix_
     key j is slot j % page_size of page block_table[b, j // page_size] (int32 [batch, width]); prefix keys lie in
     prefix_pages (int32) the same way.  A token that sees no key gets zeros; rows from q_offsets[-1] on are left as
     they are.  Values that some new token of a sequence sees and another does not must be finite.  max_q: the
-    usual number of new tokens of a sequence -- it shapes the launch, any value is right.
+    usual number of new tokens of a sequence -- it shapes the launch, any value is right: while max_q * G is below 64, the
+    prefix is read for tiles of up to 128 rows from all sequences; from there on by the tiles of each sequence.
 
     Lengths, tables and offsets stay on the device and are read by every launch, so a captured CUDA graph
     follows them; only prefix_len and the shapes are fixed at capture.  A page outside the cache reads as zeros, a
@@ -760,7 +761,8 @@ def sample_tokens(logits, u, out, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     top_k > 0 keeps the k largest logits, top_p < 1 of those, in descending order, every one before which less than
     top_p of their mass lies, min_p > 0 of those the ones with w_i >= min_p; the token is the first kept index, in
     index order, whose inclusive sum of w exceeds u times the kept sum.  temperature 0: the largest logit.
-    Ties go to the lowest index.  NaN and -inf are never chosen; a row of nothing else gives -1."""
+    Ties go to the lowest index.  NaN and -inf are never chosen; a row of nothing else gives -1.  Weights are good to a
+    relative 2^-37, sums to 64 bits."""
     lib = _lib.load()
     tens = [v if isinstance(v, torch.Tensor) else None for v in (temperature, top_k, top_p, min_p)]
     if _on_host(logits, u, out, *tens):

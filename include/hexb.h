@@ -336,9 +336,11 @@ int hexb_paged_attention_f16(const hexb_paged_attention_desc *desc, void *worksp
  *   min_p > 0     keeps those with w_i >= min_p (at most 1 counts);
  *   out = the first kept index, in index order, whose inclusive sum of w exceeds u * (sum of the kept w).
  * Ties rank by index, the lower one first.  NaN and -inf are never chosen; a row of nothing else gives -1.
- * +inf: only the rows' +inf entries have weight.  u outside [0, 1) is clamped.  Weights and sums are formed in 64 bits, and
- * the result does not depend on the order of atomics.  The parameters are device arrays of `rows` entries, or NULL
- * for the scalar that follows (temperature0, ...).  vocab <= 2^28. */
+ * +inf: only the rows' +inf entries have weight.  u outside [0, 1) is clamped.  Weights have a relative error below 2^-37 and
+ * are summed in 64 bits: the token is the definition's wherever u and top_p lie farther from a border than 2^-35 of the
+ * mass (2^-31 from 2^24 logits on), and min_p farther from a weight than 2^-37 of it.  Equal inputs give equal tokens: the
+ * order of atomics has no say.  The parameters are device arrays of `rows` entries, or NULL for the scalar that follows
+ * (temperature0, ...).  vocab <= 2^28. */
 int hexb_sample_tokens(int dtype, const void *logits, const float *u, int64_t *out, int64_t rows, int64_t vocab,
                        int64_t row_stride, const float *temperature, const int32_t *top_k, const float *top_p,
                        const float *min_p, float temperature0, int top_k0, float top_p0, float min_p0, void *stream);
